@@ -10,6 +10,7 @@ LinearAttentionResumable (state carried across calls), LinearAttentionNormalized
 denominator fused into streaming kernels) and host.HostPipeline (pinned host tensors).
 """
 from .functions import (
+    GatedLinearRecurrence,
     LinearAttention,
     LinearAttentionNormalized,
     LinearAttentionResumable,
@@ -33,6 +34,7 @@ __all__ = [
     "LinearAttentionResumable",
     "LinearAttentionNormalized",
     "TaylorLinearAttention",
+    "GatedLinearRecurrence",
     "linear_flash_wrapper_fwd",
     "linear_flash_wrapper_bwd",
     "linear_flash_wrapper_fwd_smallv_hd",

@@ -20,6 +20,7 @@ FLA_DEBUG_FORCE_SINGLE_SWEEP = 4
 FLA_MAX_RANKS = 8
 FLA_DTYPE_BF16 = 0
 FLA_DTYPE_F16 = 1
+FLA_DTYPE_F32 = 2
 
 
 class FlaTensor(ctypes.Structure):
@@ -62,6 +63,30 @@ class FlaArgs(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("wait_limit_us", ctypes.c_uint32),
         ("debug_flags", ctypes.c_uint32),
+    ]
+
+
+class FlaRecurrenceArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("seqlen", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("g_dtype", ctypes.c_int32),
+        ("x", FlaTensor),
+        ("g", FlaTensor),
+        ("o", FlaTensor),
+        ("d_o", FlaTensor),
+        ("d_x", FlaTensor),
+        ("d_g", FlaTensor),
+        ("s_init", ctypes.c_void_p),
+        ("s_final", ctypes.c_void_p),
+        ("r_init", ctypes.c_void_p),
+        ("r_final", ctypes.c_void_p),
+        ("states", ctypes.c_void_p),
+        ("states_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
     ]
 
 
@@ -120,6 +145,9 @@ EXPORTED_SYMBOLS = (
     "fla_sm100_exchange_close",
     "fla_sm100_exchange_free",
     "fla_sm100_last_launch_count",
+    "fla_sm100_recurrence_states_bytes",
+    "fla_sm100_recurrence_fwd",
+    "fla_sm100_recurrence_bwd",
 )
 
 _lib = None
@@ -217,6 +245,9 @@ def load() -> ctypes.CDLL:
     lib.fla_sm100_state_exchange.restype = ctypes.c_int
     lib.fla_sm100_state_exchange.argtypes = [ctypes.POINTER(FlaArgs), ctypes.c_int, ctypes.POINTER(FlaExchange)]
     lib.fla_sm100_last_launch_count.restype = ctypes.c_int
+    lib.fla_sm100_recurrence_states_bytes.restype = ctypes.c_size_t
+    for name in ("fla_sm100_recurrence_states_bytes", "fla_sm100_recurrence_fwd", "fla_sm100_recurrence_bwd"):
+        getattr(lib, name).argtypes = [ctypes.POINTER(FlaRecurrenceArgs)]
     if lib.fla_sm100_abi_version() != FLA_ABI_VERSION:
         raise ImportError("libflashlinear_sm100.so has a different ABI version; rebuild it")
     _lib = lib

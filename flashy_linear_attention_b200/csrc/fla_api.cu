@@ -19,6 +19,7 @@
 #include "fla_taylor.cuh"
 #include "fla_taylor_attention.cuh"
 #include "fla_decode.cuh"
+#include "fla_internal.h"
 
 #include <cuda_runtime.h>
 
@@ -28,8 +29,13 @@
 #include <cstdlib>
 #include <cstring>
 
+namespace fla {
+thread_local int g_last_launches = 0;
+}
+
 namespace {
 
+using fla::g_last_launches;
 using fla::KernelParams;
 using fla::Problem;
 
@@ -58,7 +64,6 @@ EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-thread_local int g_last_launches = 0;
 // Bounded-wait limit (units of 1024 SM cycles, 0 = default) and the wait-timeout test hook of the
 // call in progress on this thread; check_common() sets them from FlaArgs.
 thread_local unsigned g_wait_limit_us = 0;

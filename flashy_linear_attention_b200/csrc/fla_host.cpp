@@ -403,6 +403,90 @@ std::optional<std::array<Tensor, 3>> taylor_backward_in_memory(const Tensor& g, 
   return std::array<Tensor, 3>{raw((*r)[0], q), raw((*r)[1], k), (*r)[2]};
 }
 
+// The gated linear recurrence. Tensors are read where they are; neighbouring columns have to be neighbours in memory.
+bool recurrence_rows(const Tensor& t) {
+  return t.layout() == at::kStrided && t.dim() == 4 && t.is_cuda() && !t.is_neg() && (t.stride(3) == 1 || t.size(3) == 1);
+}
+int float_type(const Tensor& t) {
+  const auto s = t.scalar_type();
+  return s == at::kBFloat16 ? FLA_DTYPE_BF16 : s == at::kHalf ? FLA_DTYPE_F16 : s == at::kFloat ? FLA_DTYPE_F32 : -1;
+}
+bool recurrence_covered(const Tensor& x, const Tensor& g) {
+  if (!recurrence_rows(x) || !recurrence_rows(g) || x.sizes() != g.sizes() || x.device() != g.device() || x.numel() == 0)
+    return false;
+  if (float_type(x) < 0 || (float_type(g) != float_type(x) && float_type(g) != FLA_DTYPE_F32)) return false;
+  for (int d = 0; d < 4; ++d)
+    if (x.size(d) > INT32_MAX) return false;
+  return true;
+}
+bool channel_state(const OptTensor& s, const Tensor& x) {
+  return !s.has_value() || (s->is_cuda() && s->device() == x.device() && s->scalar_type() == at::kFloat && s->dim() == 3 &&
+                            s->size(0) == x.size(0) && s->size(1) == x.size(1) && s->size(2) == x.size(3) &&
+                            s->is_contiguous() && !s->is_neg());
+}
+Tensor rows_like(const Tensor& t) {
+  const Tensor out = at::empty_like(t);
+  return recurrence_rows(out) ? out : at::empty(t.sizes(), t.options());
+}
+FlaRecurrenceArgs recurrence_args(const Tensor& x, const Tensor& g) {
+  FlaRecurrenceArgs a = {};
+  a.batch = static_cast<int32_t>(x.size(0));
+  a.heads = static_cast<int32_t>(x.size(1));
+  a.seqlen = static_cast<int32_t>(x.size(2));
+  a.dim = static_cast<int32_t>(x.size(3));
+  a.dtype = float_type(x);
+  a.g_dtype = float_type(g);
+  a.x = desc(x);
+  a.g = desc(g);
+  a.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+  return a;
+}
+struct Recurrence {
+  Tensor out, s_final;
+  OptTensor states;
+};
+std::optional<Recurrence> recurrence_forward(const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states) {
+  if (!recurrence_covered(x, g) || !channel_state(s_init, x)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  FlaRecurrenceArgs a = recurrence_args(x, g);
+  Recurrence r{rows_like(x), at::empty({x.size(0), x.size(1), x.size(3)}, x.options().dtype(at::kFloat)), std::nullopt};
+  a.o = desc(r.out);
+  if (s_init.has_value()) a.s_init = s_init->data_ptr<float>();
+  a.s_final = r.s_final.data_ptr<float>();
+  if (keep_states) {
+    a.states_bytes = fla_sm100_recurrence_states_bytes(&a);
+    r.states = at::empty({static_cast<int64_t>(a.states_bytes)}, x.options().dtype(at::kByte));
+    a.states = r.states->data_ptr();
+  }
+  check(fla_sm100_recurrence_fwd(&a), "fla_sm100_recurrence_fwd");
+  return r;
+}
+std::optional<std::array<OptTensor, 3>> recurrence_backward(const OptTensor& dy, const Tensor& x, const Tensor& g,
+                                                            const OptTensor& states, const OptTensor& ds, bool need_x,
+                                                            bool need_g, bool need_s) {
+  if (!recurrence_covered(x, g) || !channel_state(ds, x) || !states.has_value() || !states->is_cuda() ||
+      states->device() != x.device() || !states->is_contiguous() || !(need_x || need_g || need_s))
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  FlaRecurrenceArgs a = recurrence_args(x, g);
+  Tensor rows;
+  if (dy.has_value()) {
+    if (dy->sizes() != x.sizes() || dy->scalar_type() != x.scalar_type() || dy->device() != x.device()) return std::nullopt;
+    rows = recurrence_rows(*dy) ? *dy : dy->contiguous();
+    if (!recurrence_rows(rows)) return std::nullopt;
+    a.d_o = desc(rows);
+  }
+  std::array<OptTensor, 3> out;
+  if (need_x) a.d_x = desc(*(out[0] = rows_like(x)));
+  if (need_g) a.d_g = desc(*(out[1] = rows_like(g)));
+  if (need_s) a.r_final = (out[2] = at::empty({x.size(0), x.size(1), x.size(3)}, x.options().dtype(at::kFloat)))->data_ptr<float>();
+  if (ds.has_value()) a.r_init = ds->data_ptr<float>();
+  a.states = states->data_ptr();
+  a.states_bytes = static_cast<size_t>(states->numel() * states->element_size());
+  check(fla_sm100_recurrence_bwd(&a), "fla_sm100_recurrence_bwd");
+  return out;
+}
+
 // What is saved beside the repacked copy of an input that is not kept itself: an empty tensor that shares
 // its version count, for autograd to see that it was changed in place. (An inference tensor has none;
 // it is returned itself, and autograd refuses it as it always does.)
@@ -430,6 +514,25 @@ PYBIND11_MODULE(_hostcalls, m) {
     return py::make_tuple(r->out, r->s_final, r->seg_states, views);
   });
   m.def("version_of", &version_of);
+  m.def("recurrence_forward", [](const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states) -> py::object {
+    std::optional<Recurrence> r;
+    {
+      const py::gil_scoped_release unlocked;
+      r = recurrence_forward(x, g, s_init, keep_states);
+    }
+    if (!r.has_value()) return py::none();
+    return py::make_tuple(r->out, r->s_final, r->states);
+  });
+  m.def("recurrence_backward", [](const OptTensor& dy, const Tensor& x, const Tensor& g, const OptTensor& states,
+                                  const OptTensor& ds, bool need_x, bool need_g, bool need_s) -> py::object {
+    std::optional<std::array<OptTensor, 3>> r;
+    {
+      const py::gil_scoped_release unlocked;
+      r = recurrence_backward(dy, x, g, states, ds, need_x, need_g, need_s);
+    }
+    if (!r.has_value()) return py::none();
+    return py::make_tuple((*r)[0], (*r)[1], (*r)[2]);
+  });
   m.def("taylor_forward", &taylor_forward, py::call_guard<py::gil_scoped_release>());
   m.def("taylor_backward", &taylor_backward, py::call_guard<py::gil_scoped_release>());
   m.def("taylor_forward_in_memory", &taylor_forward_in_memory, py::call_guard<py::gil_scoped_release>());

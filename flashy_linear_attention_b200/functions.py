@@ -13,8 +13,9 @@ from typing import Any, Tuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import ops, recurrence
 
 
 def _autocast_to_bf16(forward):
@@ -239,3 +240,42 @@ class TaylorLinearAttention(Function):
                 return tuple(grads)
             features = ops.taylor_features(xq), ops.taylor_features(xk)
         return ops.taylor_backward_in_memory(grad_output, xq, xk, v, *features)
+
+
+class GatedLinearRecurrence(Function):
+    """Gated linear recurrence, a state of its own for every channel:
+    ``h_t = exp(log_decay_t) h_{t-1} + x_t``, ``out_t = h_t``.
+
+    ``out, s_final = GatedLinearRecurrence.apply(x, log_decay, s_init=None)`` with x and log_decay ``[B, H, N, D]``
+    (bf16, fp16 or fp32; log_decay of the same type or fp32; any strides, broadcast by ``expand`` included) and fp32
+    states ``[B, H, D]``, as ``LinearAttentionResumable`` has them: feeding ``s_final`` of one call as ``s_init`` of the
+    next gives what one call over the concatenated tokens gives, for any number of tokens a call, one and none included.
+    ``out`` is h rounded to x's type; h itself is summed in fp32. All of x, log_decay and s_init are differentiable.
+
+    ``log_decay`` is usually at most 0 (a ``logsigmoid``, or minus a rate). -inf drops the state, whatever it holds: set
+    it on the first token of each document of a packed row, and nothing passes between them, in either pass. 0, with x = 0,
+    passes a token over, as for padding. Under autocast x is cast to bf16 as in the other Functions, log_decay unless it is
+    fp32; the states stay fp32.
+
+    The reference has no counterpart.
+    """
+
+    @staticmethod
+    def forward(ctx: Any, x, log_decay, s_init=None):
+        if torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.bfloat16)
+            if log_decay.dtype != torch.float32:
+                log_decay = log_decay.to(torch.bfloat16)
+        out, s_final, states = recurrence.recurrence_fwd(x, log_decay, s_init, any(ctx.needs_input_grad[:3]))
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, log_decay, states)
+        return out, s_final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_output, grad_s_final):
+        x, log_decay, states = ctx.saved_tensors
+        if grad_output is None and grad_s_final is None:
+            return None, None, None
+        needs = tuple(ctx.needs_input_grad) + (False,) * (3 - len(ctx.needs_input_grad))
+        return tuple(recurrence.recurrence_bwd(grad_output, x, log_decay, states, grad_s_final, needs)[:len(ctx.needs_input_grad)])

@@ -36,6 +36,7 @@ extern "C" {
 #define FLA_ABI_VERSION 9
 #define FLA_DTYPE_BF16 0
 #define FLA_DTYPE_F16 1
+#define FLA_DTYPE_F32 2 /* recurrence and layer norm only */
 
 enum {
   FLA_OK = 0,
@@ -341,6 +342,35 @@ int fla_sm100_taylor_features_bwd(const void* dphi, const void* x, void* dx, lon
  * from zero. Other shapes: FLA_ERR_UNSUPPORTED. The backward needs q, k, v and d_o only. No scratch. */
 int fla_sm100_taylor_fwd(const FlaArgs* args);
 int fla_sm100_taylor_bwd(const FlaArgs* args);
+
+/* ---- gated linear recurrence ----
+ * h_t = exp(g_t) h_(t-1) + x_t for every channel of [batch, heads, seqlen, dim] tensors, out_t = h_t. g_t = -inf drops the
+ * state, whatever it holds (a document starts); g_t = 0 and x_t = 0 leave it as it is (a token to be passed over).
+ * The reference has no counterpart. Tensors have any (batch, head, token) strides, zero for broadcast inputs included,
+ * and an innermost stride of 1; nothing has to be aligned beyond its element size. States are fp32
+ * [batch, heads, dim], contiguous. dtype is that of x, o, d_o and d_x, g_dtype that of g and d_g: the same or fp32.
+ * fwd reads x, g and s_init (null: zero), writes o and, unless null, s_final and `states`: the state before every
+ * few tokens, of recurrence_states_bytes(), 16-byte aligned, private to the library, for the backward of the same x and g.
+ * bwd reads x, g, d_o (null: zero), r_init (gradient of s_final, null: zero) and `states`, writes d_x, d_g and
+ * r_final (gradient of s_init), each unless null. Gates must not make the state overflow fp32 within a sequence.
+ * No scratch; one launch; sums in an order that depends on the shapes and strides only. */
+typedef struct FlaRecurrenceArgs {
+  int32_t batch, heads, seqlen, dim;
+  int32_t dtype, g_dtype;
+  FlaTensor x, g;
+  FlaTensor o;
+  FlaTensor d_o, d_x, d_g;
+  const float* s_init;
+  float* s_final;
+  const float* r_init;
+  float* r_final;
+  void* states;
+  size_t states_bytes;
+  void* stream;
+} FlaRecurrenceArgs;
+size_t fla_sm100_recurrence_states_bytes(const FlaRecurrenceArgs* args);
+int fla_sm100_recurrence_fwd(const FlaRecurrenceArgs* args);
+int fla_sm100_recurrence_bwd(const FlaRecurrenceArgs* args);
 
 /* Forward pass for callers that cannot obtain device memory themselves.
  * It has no counterpart in the reference (whose wrappers allocate through torch).
