@@ -86,7 +86,10 @@ class FlaRecurrenceArgs(ctypes.Structure):
         ("r_final", ctypes.c_void_p),
         ("states", ctypes.c_void_p),
         ("states_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
         ("stream", ctypes.c_void_p),
+        ("wait_limit_us", ctypes.c_uint32),
+        ("debug_flags", ctypes.c_uint32),
     ]
 
 

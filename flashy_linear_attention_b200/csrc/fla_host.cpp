@@ -428,7 +428,7 @@ Tensor rows_like(const Tensor& t) {
   const Tensor out = at::empty_like(t);
   return recurrence_rows(out) ? out : at::empty(t.sizes(), t.options());
 }
-FlaRecurrenceArgs recurrence_args(const Tensor& x, const Tensor& g) {
+FlaRecurrenceArgs recurrence_args(const Tensor& x, const Tensor& g, unsigned debug_flags, uintptr_t status) {
   FlaRecurrenceArgs a = {};
   a.batch = static_cast<int32_t>(x.size(0));
   a.heads = static_cast<int32_t>(x.size(1));
@@ -438,6 +438,8 @@ FlaRecurrenceArgs recurrence_args(const Tensor& x, const Tensor& g) {
   a.g_dtype = float_type(g);
   a.x = desc(x);
   a.g = desc(g);
+  a.debug_flags = debug_flags;
+  a.status = reinterpret_cast<int32_t*>(status);
   a.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
   return a;
 }
@@ -445,10 +447,11 @@ struct Recurrence {
   Tensor out, s_final;
   OptTensor states;
 };
-std::optional<Recurrence> recurrence_forward(const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states) {
+std::optional<Recurrence> recurrence_forward(const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states,
+                                             unsigned debug_flags, uintptr_t status) {
   if (!recurrence_covered(x, g) || !channel_state(s_init, x)) return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
-  FlaRecurrenceArgs a = recurrence_args(x, g);
+  FlaRecurrenceArgs a = recurrence_args(x, g, debug_flags, status);
   Recurrence r{rows_like(x), at::empty({x.size(0), x.size(1), x.size(3)}, x.options().dtype(at::kFloat)), std::nullopt};
   a.o = desc(r.out);
   if (s_init.has_value()) a.s_init = s_init->data_ptr<float>();
@@ -463,12 +466,12 @@ std::optional<Recurrence> recurrence_forward(const Tensor& x, const Tensor& g, c
 }
 std::optional<std::array<OptTensor, 3>> recurrence_backward(const OptTensor& dy, const Tensor& x, const Tensor& g,
                                                             const OptTensor& states, const OptTensor& ds, bool need_x,
-                                                            bool need_g, bool need_s) {
+                                                            bool need_g, bool need_s, unsigned debug_flags, uintptr_t status) {
   if (!recurrence_covered(x, g) || !channel_state(ds, x) || !states.has_value() || !states->is_cuda() ||
       states->device() != x.device() || !states->is_contiguous() || !(need_x || need_g || need_s))
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
-  FlaRecurrenceArgs a = recurrence_args(x, g);
+  FlaRecurrenceArgs a = recurrence_args(x, g, debug_flags, status);
   Tensor rows;
   if (dy.has_value()) {
     if (dy->sizes() != x.sizes() || dy->scalar_type() != x.scalar_type() || dy->device() != x.device()) return std::nullopt;
@@ -514,21 +517,23 @@ PYBIND11_MODULE(_hostcalls, m) {
     return py::make_tuple(r->out, r->s_final, r->seg_states, views);
   });
   m.def("version_of", &version_of);
-  m.def("recurrence_forward", [](const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states) -> py::object {
+  m.def("recurrence_forward", [](const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states,
+                                 unsigned debug_flags, uintptr_t status) -> py::object {
     std::optional<Recurrence> r;
     {
       const py::gil_scoped_release unlocked;
-      r = recurrence_forward(x, g, s_init, keep_states);
+      r = recurrence_forward(x, g, s_init, keep_states, debug_flags, status);
     }
     if (!r.has_value()) return py::none();
     return py::make_tuple(r->out, r->s_final, r->states);
   });
   m.def("recurrence_backward", [](const OptTensor& dy, const Tensor& x, const Tensor& g, const OptTensor& states,
-                                  const OptTensor& ds, bool need_x, bool need_g, bool need_s) -> py::object {
+                                  const OptTensor& ds, bool need_x, bool need_g, bool need_s, unsigned debug_flags,
+                                  uintptr_t status) -> py::object {
     std::optional<std::array<OptTensor, 3>> r;
     {
       const py::gil_scoped_release unlocked;
-      r = recurrence_backward(dy, x, g, states, ds, need_x, need_g, need_s);
+      r = recurrence_backward(dy, x, g, states, ds, need_x, need_g, need_s, debug_flags, status);
     }
     if (!r.has_value()) return py::none();
     return py::make_tuple((*r)[0], (*r)[1], (*r)[2]);

@@ -46,11 +46,14 @@ struct RecurrenceParams {
   float* end;                 // [bh][c]: state after the last token, resp. R_0; null: not wanted
   float* states;              // [b][run][heads * c]: the state before each run; null: not wanted (forward)
   int heads, n, c;
+  int* status;
+  unsigned long long wait_limit_ns;
+  int withhold;               // the first map of rank 0 is never sent (a test of the wait's limit)
   int tiles;                  // tiles of channels a (batch, head)
   long long tiles_all;
 };
 
-constexpr int kRecThreads = 256;
+constexpr int kShortThreads = 128;
 constexpr int kRecMaxCluster = 8;
 
 // Tokens a thread holds: a run. 16-bit rows and gates leave room for twice as many.
@@ -63,238 +66,171 @@ struct RunMap {
 };
 
 __device__ __forceinline__ float apply_map(float c, float hi, float lo, float b) {
-  // (from zero the map is b, also where a growing gate has overflowed; the correction of an infinite state is NaN)
-  if (hi < 0.f || c == 0.f) return b;
-  return fmaf(hi, c, fabsf(c) <= 3.4e38f ? fmaf(lo, c, b) : b);
+  const float low = fabsf(c) <= 3.4e38f ? fmaf(lo, c, b) : b;  // (two opposite infinities would make a NaN)
+  return hi < 0.f ? b : fmaf(hi, c, low);
 }
 __device__ __forceinline__ float2 apply_map(float2 c, const RunMap& m) {
   return make_float2(apply_map(c.x, m.hi.x, m.lo.x, m.b.x), apply_map(c.y, m.hi.y, m.lo.y, m.b.y));
 }
 
-// A decay that would round to zero (the smallest normal number): what it adds is below 2^-126 of the state, but an
-// infinity stays one until a gate of minus infinity, as it does token by token.
-constexpr float kLeastDecay = 1.17549435e-38f;
+// 2^x, off by 2^-22 of it; results below the normal numbers are zero.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.44269504f;
 
 // exp(s) as hi + lo. Near 1, where the error of one float would act on a long memory, the second takes up what the
-// first lost: exp(s) - 1 from its series (s^7 / 5040 is below 2^-31 of it there).
+// first lost: exp(s) - 1 from its series (s^7 / 5040 is below 2^-31 of it there). Further off the memory ends within
+// eight runs, and the fast exponential will do.
 __device__ __forceinline__ void split_exp(float s, float* hi, float* lo) {
-  if (s == -INFINITY) {
-    *hi = -1.f;
-    *lo = 0.f;
-    return;
-  }
   float e = fmaf(s, 1.f / 720.f, 1.f / 120.f);
   e = fmaf(s, e, 1.f / 24.f);
   e = fmaf(s, e, 1.f / 6.f);
   e = fmaf(s, e, 0.5f);
   e = fmaf(s * s, e, s);
   const bool near = fabsf(s) < 0.125f;
-  *hi = near ? 1.f + e : fmaxf(expf(s), kLeastDecay);
+  *hi = near ? 1.f + e : s == -INFINITY ? -1.f : fast_exp2(s * kLog2e);
   *lo = near ? e - (*hi - 1.f) : 0.f;
 }
-
-// Decay of one token. 16-bit rows: the fast exponential, off by 2^-22 or so, which acts on 16 tokens at most.
-template <typename TX>
-__device__ __forceinline__ float decay(float g) {
-  return sizeof(TX) == 4 ? expf(g) : __expf(g);
+// The factor of a run is kept inside the normal numbers: below, what it adds is less than 2^-126 of the state, but an
+// infinity stays one until a gate of minus infinity, as it does token by token; above, a state of zero stays zero.
+constexpr float kLeastDecay = 1.17549435e-38f, kMostDecay = 3.40282347e38f;
+__device__ __forceinline__ float normal(float hi) {
+  return fabsf(hi) < kLeastDecay ? kLeastDecay : hi > kMostDecay ? kMostDecay : hi;
 }
-template <typename TX>
-__device__ __forceinline__ float advance(float g, float h, float x) {
-  return g == -INFINITY ? x : fmaf(decay<TX>(g), h, x);
+__device__ __forceinline__ RunMap token_map(float2 g, float2 b) {
+  RunMap m;
+  m.b = b;
+  split_exp(g.x, &m.hi.x, &m.lo.x);
+  split_exp(g.y, &m.hi.y, &m.lo.y);
+  return m;
+}
+__device__ __forceinline__ RunMap run_map(float2 sum, float2 b) {
+  RunMap m = token_map(sum, b);
+  m.hi = make_float2(normal(m.hi.x), normal(m.hi.y));
+  return m;
 }
 
-// Composition: first m, then n.
-__device__ __forceinline__ void then_map(float& hi, float& lo, float& b, float nhi, float nlo, float nb) {
-  b = apply_map(b, nhi, nlo, nb);
-  if (hi < 0.f || nhi < 0.f) {
-    hi = -1.f;
-    lo = 0.f;
-    return;
+// Two channels at once: sm_100 multiplies and adds pairs of floats in one instruction.
+__device__ __forceinline__ uint64_t bits(float2 v) { return *reinterpret_cast<const uint64_t*>(&v); }
+__device__ __forceinline__ float2 floats(uint64_t v) { return *reinterpret_cast<const float2*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return floats(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return floats(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return floats(d);
+}
+
+// Decays of one token. 16-bit rows: the fast exponential, whose error acts on the tokens of a run only.
+template <typename TX>
+__device__ __forceinline__ float2 decay(float2 g) {
+  if (sizeof(TX) == 4) return make_float2(expf(g.x), expf(g.y));
+  const float2 e = mul2(g, make_float2(kLog2e, kLog2e));
+  return make_float2(fast_exp2(e.x), fast_exp2(e.y));
+}
+// DROPS: some gate of the run is minus infinity; the state before it goes even if it is not finite.
+template <typename TX, bool DROPS>
+__device__ __forceinline__ float2 advance(float2 g, float2 h, float2 x) {
+  float2 r = fma2(decay<TX>(g), h, x);
+  if (DROPS) {
+    if (g.x == -INFINITY) r.x = x.x;
+    if (g.y == -INFINITY) r.y = x.y;
   }
-  const float p = hi * nhi;
-  lo = fmaf(hi, nhi, -p) + fmaf(hi, nlo, lo * nhi);
-  hi = fmaxf(p, kLeastDecay);
+  return r;
 }
-
-template <int LPR>
-struct RecurrenceShared {
-  RunMap run[2][kRecThreads];          // [step parity][run of the CTA][lane]
-  RunMap cta[2][kRecMaxCluster][LPR];  // [step parity][CTA of the cluster][lane]
-};
-struct Nothing {};
+// The same step backward: exp(g) times what has come together at the token.
+template <typename TX, bool DROPS>
+__device__ __forceinline__ float2 retreat(float2 g, float2 all) {
+  float2 r = mul2(decay<TX>(g), all);
+  if (DROPS) {
+    if (g.x == -INFINITY) r.x = 0.f;
+    if (g.y == -INFINITY) r.y = 0.f;
+  }
+  return r;
+}
 
 struct Place {  // what a thread works on
-  long long tile;
-  int lane, run, runs, rank, ranks;
   int b, h, c0, gap;
   bool ok0, ok1;
 };
-
-// Exchanges the maps of a step. `carry` is the state before the cluster's step and becomes the one behind it; returns
-// the state before this thread's run. `order`: position of the run among the CTA's, of the CTA among the cluster's, in
-// the direction of the walk.
-template <int LPR>
-__device__ __forceinline__ float2 exchange(RecurrenceShared<LPR>& sh, int parity, const RunMap& mine, const Place& w,
-                                           float2& carry) {
-  const int run = w.run, runs = w.runs, lane = w.lane, rank = w.rank, ranks = w.ranks;
-  RunMap* maps = sh.run[parity];
-  maps[run * LPR + lane] = mine;
-  __syncthreads();
-  float2 c = carry, before = carry;
-  if (ranks == 1) {
-#pragma unroll 4
-    for (int r = 0; r < runs; ++r) {
-      if (r == run) before = c;
-      c = apply_map(c, maps[r * LPR + lane]);
-    }
-    carry = c;
-    return before;
-  }
-  cg::cluster_group cluster = cg::this_cluster();
-  if (run == 0) {
-    RunMap all = maps[lane];
-    for (int r = 1; r < runs; ++r) {
-      const RunMap m = maps[r * LPR + lane];
-      then_map(all.hi.x, all.lo.x, all.b.x, m.hi.x, m.lo.x, m.b.x);
-      then_map(all.hi.y, all.lo.y, all.b.y, m.hi.y, m.lo.y, m.b.y);
-    }
-    for (int r = 0; r < ranks; ++r)  // (cluster ranks and the order of the walk are the same)
-      *cluster.map_shared_rank(&sh.cta[parity][rank][lane], r) = all;
-  }
-  // A CTA overwrites what it wrote two steps ago, which its peers have read before they came to the barrier of the step
-  // between; after the last barrier nobody writes to a peer, so a CTA may leave.
-  cluster.sync();
-  for (int r = 0; r < ranks; ++r) {
-    if (r == rank) before = c;
-    c = apply_map(c, sh.cta[parity][r][lane]);
-  }
-  carry = c;
-  c = before;
-  for (int r = 0; r < run; ++r) c = apply_map(c, maps[r * LPR + lane]);
-  return c;
-}
-
-// ALONE: every group of LPR lanes has a tile and all its tokens to itself (short sequences: nothing to exchange).
-template <bool PAIR, int LPR, bool ALONE>
-__device__ __forceinline__ Place place(const RecurrenceParams& p) {
+template <bool PAIR, int LPR>
+__device__ __forceinline__ Place place(const RecurrenceParams& p, long long tile, int lane) {
   Place w;
-  w.lane = threadIdx.x % LPR;
-  const int group = threadIdx.x / LPR, groups = blockDim.x / LPR;
-  if (ALONE) {
-    w.run = w.rank = 0;
-    w.runs = w.ranks = 1;
-    w.tile = static_cast<long long>(blockIdx.x) * groups + group;
-  } else {
-    cg::cluster_group cluster = cg::this_cluster();
-    w.run = group;
-    w.runs = groups;
-    w.ranks = cluster.num_blocks();
-    w.rank = cluster.block_rank();
-    w.tile = blockIdx.x / w.ranks;
-  }
-  const long long bh = w.tile / p.tiles;
+  const long long bh = tile / p.tiles;
   w.b = static_cast<int>(bh / p.heads);
   w.h = static_cast<int>(bh % p.heads);
   w.gap = PAIR ? 1 : LPR;
-  w.c0 = static_cast<int>(w.tile % p.tiles) * 2 * LPR + (PAIR ? 2 * w.lane : w.lane);
-  w.ok0 = w.c0 < p.c && w.tile < p.tiles_all;
-  w.ok1 = w.c0 + w.gap < p.c && w.tile < p.tiles_all;
+  w.c0 = static_cast<int>(tile % p.tiles) * 2 * LPR + (PAIR ? 2 * lane : lane);
+  w.ok0 = w.c0 < p.c;
+  w.ok1 = w.c0 + w.gap < p.c;
   return w;
 }
-
 // Index into RecurrenceParams::states, whose layout does not depend on how heads were joined.
 __device__ __forceinline__ long long state_of(const RecurrenceParams& p, const Place& w, int run, int runs_all) {
   return ((static_cast<long long>(w.b) * runs_all + run) * p.heads + w.h) * p.c + w.c0;
 }
+
+// ------------------------------------------------------------------------------------------------------------
+// Short sequences, and rows so far apart that their offsets need 64 bits: every group of LPR lanes walks a tile of
+// channels alone, token by token. A program that decodes multiplies its state once a call by one token's decay, so
+// that is split in two floats here.
 
 template <typename T>
 __device__ __forceinline__ T* row0(const RecurrenceTensor& t, const Place& w) {
   return static_cast<T*>(t.ptr) + w.b * t.sb + w.h * t.sh + w.c0;
 }
 
-template <typename TX, typename TG, bool PAIR, int LPR, bool ALONE>
-__global__ void __launch_bounds__(kRecThreads, 2) fla_recurrence_fwd_kernel(const RecurrenceParams p) {
+template <typename TX, typename TG, bool PAIR, int LPR>
+__global__ void __launch_bounds__(kShortThreads) fla_recurrence_short_fwd_kernel(const RecurrenceParams p) {
   constexpr int T = kRunTokens<TX, TG>;
-  __shared__ std::conditional_t<ALONE, Nothing, RecurrenceShared<LPR>> sh;
-  const Place w = place<PAIR, LPR, ALONE>(p);
-  if (ALONE && !w.ok0) return;
+  const long long tile = static_cast<long long>(blockIdx.x) * (kShortThreads / LPR) + threadIdx.x / LPR;
+  if (tile >= p.tiles_all) return;
+  const Place w = place<PAIR, LPR>(p, tile, threadIdx.x % LPR);
   const TX* xp = row0<const TX>(p.x, w);
   const TG* gp = row0<const TG>(p.g, w);
   TX* op = row0<TX>(p.o, w);
   const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
-  float2 carry = make_float2(0.f, 0.f);
-  if (p.start != nullptr) carry = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
-
-  typename PairOf<TX>::Raw x[T], x_next[T];
-  typename PairOf<TG>::Raw g[T], g_next[T];
-  const int span = w.ranks * w.runs * T;  // tokens a step
-  const int steps = (p.n - 1) / span + 1;
-  auto fetch = [&](int t0, auto& xr, auto& gr) {
+  const int runs_all = (p.n - 1) / T + 1;
+  float2 h = make_float2(0.f, 0.f);
+  if (p.start != nullptr) h = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
+  for (int run = 0; run < runs_all; ++run) {
+    const int t0 = run * T;
+    if (p.states != nullptr) store_pair<float, PAIR>(p.states + state_of(p, w, run, runs_all), w.gap, w.ok0, w.ok1, h);
+    typename PairOf<TX>::Raw x[T];
+    typename PairOf<TG>::Raw g[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const bool in = t0 + t < p.n;
-      xr[t] = load_pair<TX, PAIR>(xp + (t0 + t) * p.x.sn, w.gap, w.ok0 && in, w.ok1 && in);
-      gr[t] = load_pair<TG, PAIR>(gp + (t0 + t) * p.g.sn, w.gap, w.ok0 && in, w.ok1 && in);
+      x[t] = load_pair<TX, PAIR>(xp + (t0 + t) * p.x.sn, w.gap, w.ok0 && in, w.ok1 && in);
+      g[t] = load_pair<TG, PAIR>(gp + (t0 + t) * p.g.sn, w.gap, w.ok0 && in, w.ok1 && in);
     }
-  };
-  const int first = (w.rank * w.runs + w.run) * T;
-  fetch(first, x, g);
-  if (!ALONE && w.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
-  for (int step = 0; step < steps; ++step) {
-    const int t0 = step * span + first;
-    if (step + 1 < steps) fetch(t0 + span, x_next, g_next);
-    float2 h = carry;
-    if constexpr (!ALONE) {
-      h = make_float2(0.f, 0.f);
-      float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const float2 xv = unpack_pair<TX>(x[t]), gv = unpack_pair<TG>(g[t]);
-        sum.x += gv.x;
-        sum.y += gv.y;
-        h.x = advance<TX>(gv.x, h.x, xv.x);
-        h.y = advance<TX>(gv.y, h.y, xv.y);
-      }
-      RunMap m;
-      m.b = h;
-      split_exp(sum.x, &m.hi.x, &m.lo.x);
-      split_exp(sum.y, &m.hi.y, &m.lo.y);
-      h = exchange<LPR>(sh, step & 1, m, w, carry);
-    }
-    if (p.states != nullptr && t0 < p.n)
-      store_pair<float, PAIR>(p.states + state_of(p, w, t0 / T, (p.n - 1) / T + 1), w.gap, w.ok0, w.ok1, h);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      const float2 xv = unpack_pair<TX>(x[t]), gv = unpack_pair<TG>(g[t]);
-      if constexpr (ALONE) {  // (a program that decodes multiplies its state once a call, by one token's decay)
-        RunMap m;
-        m.b = xv;
-        split_exp(gv.x, &m.hi.x, &m.lo.x);
-        split_exp(gv.y, &m.hi.y, &m.lo.y);
-        h = apply_map(h, m);
-      } else {
-        h.x = advance<TX>(gv.x, h.x, xv.x);
-        h.y = advance<TX>(gv.y, h.y, xv.y);
-      }
-      const bool in = t0 + t < p.n;
-      store_pair<TX, PAIR>(op + (t0 + t) * p.o.sn, w.gap, w.ok0 && in, w.ok1 && in, h);
-    }
-    if (ALONE) carry = h;
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      x[t] = x_next[t];
-      g[t] = g_next[t];
+      if (t0 + t >= p.n) break;
+      h = apply_map(h, token_map(unpack_pair<TG>(g[t]), unpack_pair<TX>(x[t])));
+      store_pair<TX, PAIR>(op + (t0 + t) * p.o.sn, w.gap, w.ok0, w.ok1, h);
     }
   }
-  if (p.end != nullptr && w.run == 0 && w.rank == 0) store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
+  if (p.end != nullptr) store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, h);
 }
 
-template <typename TX, typename TG, bool PAIR, int LPR, bool ALONE>
-__global__ void __launch_bounds__(kRecThreads, 2) fla_recurrence_bwd_kernel(const RecurrenceParams p) {
+template <typename TX, typename TG, bool PAIR, int LPR>
+__global__ void __launch_bounds__(kShortThreads) fla_recurrence_short_bwd_kernel(const RecurrenceParams p) {
   constexpr int T = kRunTokens<TX, TG>;
-  __shared__ std::conditional_t<ALONE, Nothing, RecurrenceShared<LPR>> sh;
-  const Place w = place<PAIR, LPR, ALONE>(p);
-  if (ALONE && !w.ok0) return;
+  const long long tile = static_cast<long long>(blockIdx.x) * (kShortThreads / LPR) + threadIdx.x / LPR;
+  if (tile >= p.tiles_all) return;
+  const Place w = place<PAIR, LPR>(p, tile, threadIdx.x % LPR);
   const TX* xp = row0<const TX>(p.x, w);
   const TG* gp = row0<const TG>(p.g, w);
   const TX* yp = row0<const TX>(p.o, w);
@@ -302,21 +238,14 @@ __global__ void __launch_bounds__(kRecThreads, 2) fla_recurrence_bwd_kernel(cons
   TG* dgp = row0<TG>(p.dg, w);
   const bool has_dy = p.o.ptr != nullptr;
   const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
-  float2 carry = make_float2(0.f, 0.f);
-  if (p.start != nullptr) carry = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
-
   const int runs_all = (p.n - 1) / T + 1;
-  const int span = w.ranks * w.runs;  // runs a step
-  if (!ALONE && w.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
-  const int steps = (runs_all - 1) / span + 1;
-  for (int step = 0; step < steps; ++step) {
-    // the walk starts at the end; its first runs may lie behind the last token and are the identity
-    const int run = steps * span - 1 - ((step * w.ranks + w.rank) * w.runs + w.run);
+  float2 r = make_float2(0.f, 0.f);
+  if (p.start != nullptr) r = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
+  for (int run = runs_all - 1; run >= 0; --run) {
     const int t0 = run * T;
     typename PairOf<TX>::Raw x[T], y[T];
     typename PairOf<TG>::Raw g[T];
-    float2 h = make_float2(0.f, 0.f);
-    if (run < runs_all) h = load_pair<float, PAIR>(p.states + state_of(p, w, run, runs_all), w.gap, w.ok0, w.ok1);
+    float2 h = load_pair<float, PAIR>(p.states + state_of(p, w, run, runs_all), w.gap, w.ok0, w.ok1);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const bool in = t0 + t < p.n;
@@ -324,48 +253,441 @@ __global__ void __launch_bounds__(kRecThreads, 2) fla_recurrence_bwd_kernel(cons
       g[t] = load_pair<TG, PAIR>(gp + (t0 + t) * p.g.sn, w.gap, w.ok0 && in, w.ok1 && in);
       y[t] = load_pair<TX, PAIR>(yp + (t0 + t) * p.o.sn, w.gap, w.ok0 && in && has_dy, w.ok1 && in && has_dy);
     }
-    float2 before[T];  // the state before each token
+    float2 before[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      const float2 xv = unpack_pair<TX>(x[t]), gv = unpack_pair<TG>(g[t]);
       before[t] = h;
-      h.x = advance<TX>(gv.x, h.x, xv.x);
-      h.y = advance<TX>(gv.y, h.y, xv.y);
-    }
-    float2 r = carry;
-    if constexpr (!ALONE) {
-      r = make_float2(0.f, 0.f);
-      float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int t = T - 1; t >= 0; --t) {
-        const float2 yv = unpack_pair<TX>(y[t]), gv = unpack_pair<TG>(g[t]);
-        sum.x += gv.x;
-        sum.y += gv.y;
-        r.x = gv.x == -INFINITY ? 0.f : decay<TX>(gv.x) * (yv.x + r.x);
-        r.y = gv.y == -INFINITY ? 0.f : decay<TX>(gv.y) * (yv.y + r.y);
-      }
-      RunMap m;
-      m.b = r;
-      split_exp(sum.x, &m.hi.x, &m.lo.x);
-      split_exp(sum.y, &m.hi.y, &m.lo.y);
-      r = exchange<LPR>(sh, step & 1, m, w, carry);
+      h = apply_map(h, token_map(unpack_pair<TG>(g[t]), unpack_pair<TX>(x[t])));
     }
 #pragma unroll
     for (int t = T - 1; t >= 0; --t) {
-      const float2 yv = unpack_pair<TX>(y[t]), gv = unpack_pair<TG>(g[t]);
-      const bool in = t0 + t < p.n;
-      const float2 all = make_float2(yv.x + r.x, yv.y + r.y);
-      if (p.dx.ptr != nullptr) store_pair<TX, PAIR>(dxp + (t0 + t) * p.dx.sn, w.gap, w.ok0 && in, w.ok1 && in, all);
-      const bool drop0 = gv.x == -INFINITY, drop1 = gv.y == -INFINITY;
-      r.x = drop0 ? 0.f : decay<TX>(gv.x) * all.x;
-      r.y = drop1 ? 0.f : decay<TX>(gv.y) * all.y;
+      if (t0 + t >= p.n) continue;
+      const float2 gv = unpack_pair<TG>(g[t]), all = add2(unpack_pair<TX>(y[t]), r);
+      if (p.dx.ptr != nullptr) store_pair<TX, PAIR>(dxp + (t0 + t) * p.dx.sn, w.gap, w.ok0, w.ok1, all);
+      r = apply_map(all, token_map(gv, make_float2(0.f, 0.f)));
       if (p.dg.ptr != nullptr)
-        store_pair<TG, PAIR>(dgp + (t0 + t) * p.dg.sn, w.gap, w.ok0 && in, w.ok1 && in,
-                             make_float2(drop0 ? 0.f : r.x * before[t].x, drop1 ? 0.f : r.y * before[t].y));
+        store_pair<TG, PAIR>(dgp + (t0 + t) * p.dg.sn, w.gap, w.ok0, w.ok1,
+                             make_float2(gv.x == -INFINITY ? 0.f : r.x * before[t].x, gv.y == -INFINITY ? 0.f : r.y * before[t].y));
     }
-    if (ALONE) carry = r;
   }
-  if (p.end != nullptr && w.run == 0 && w.rank == 0) store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
+  if (p.end != nullptr) store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, r);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Clusters of CTAs that walk a tile of 2 LPR channels together, a step of ranks * runs * T tokens at a time.
+
+template <int LPR, int THREADS>
+struct RecurrenceShared {
+  RunMap run[THREADS];     // [run of the CTA][lane]
+  float2 before[THREADS];  // its sum of gates, and then the state before it
+  // What the CTAs of the cluster send each other: [step parity][rank][lane], and a barrier for each parity.
+  float4 factor[2][kRecMaxCluster][LPR];  // hi, lo
+  float2 b[2][kRecMaxCluster][LPR];
+  uint64_t arrived[2];
+};
+struct Team {
+  int lane, run, rank, ranks;
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint32_t peer_address(uint32_t address, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
+  return r;
+}
+
+// Waits until the maps of all peers have arrived; false if that takes longer than the limit.
+__device__ __forceinline__ bool maps_arrived(uint32_t barrier, uint32_t phase, unsigned long long limit_ns) {
+  unsigned long long start, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(barrier), "r"(phase)
+        : "memory");
+    if (done) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (now - start > limit_ns) return false;
+  }
+}
+
+// Sends this CTA's map of a step to every CTA of the cluster, itself included, and waits for theirs. The stores count
+// their bytes at the receiver's barrier when they have arrived: unlike a barrier of the cluster, they need no fence, and
+// so do not wait for the rows that were written to memory before (5 us a step that way, 2.5 this way). A peer
+// writes to a slot again two steps later, for which it needs what this CTA sends when it has read the slot.
+template <int LPR, int THREADS>
+__device__ __forceinline__ bool trade_maps(RecurrenceShared<LPR, THREADS>& sh, int step, const RunMap& all, const Team& w,
+                                           const RecurrenceParams& p) {
+  const int parity = step & 1;
+  const uint32_t factor = shared_address(&sh.factor[parity][w.rank][w.lane]), b = shared_address(&sh.b[parity][w.rank][w.lane]);
+  const uint32_t barrier = shared_address(&sh.arrived[parity]);
+  if (w.lane == 0)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(w.ranks * LPR * 24) : "memory");
+  if (!(p.withhold && step == 0 && w.rank == 0)) {
+    for (int r = 0; r < w.ranks; ++r) {
+      const uint32_t bar = peer_address(barrier, r);
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                       peer_address(factor, r)),
+                   "f"(all.hi.x), "f"(all.hi.y), "f"(all.lo.x), "f"(all.lo.y), "r"(bar)
+                   : "memory");
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(peer_address(b, r)),
+                   "f"(all.b.x), "f"(all.b.y), "r"(bar)
+                   : "memory");
+    }
+  }
+  return maps_arrived(barrier, (step >> 1) & 1, p.wait_limit_ns);
+}
+
+// Exchanges the maps of a step and returns the state before this thread's run. `carry`, which the first run's threads
+// hold, is the state before the step and becomes the one behind it. Runs and ranks count in the direction of the walk.
+// One warp joins them: all warps doing so for themselves issued a tenth of the kernel's instructions. `lost`: a wait has
+// run out; the state is NaN from there on, and nothing is sent or waited for any more.
+template <int LPR, int THREADS>
+__device__ __forceinline__ float2 exchange(RecurrenceShared<LPR, THREADS>& sh, int step, float2 sum, float2 b, const Team& w,
+                                           const RecurrenceParams& p, float2& carry, bool& lost) {
+  constexpr int kRuns = THREADS / LPR;
+  sh.run[w.run * LPR + w.lane] = run_map(sum, b);
+  sh.before[w.run * LPR + w.lane] = sum;
+  __syncthreads();
+  if (w.run == 0) {
+    float2 c = carry;
+    if (w.ranks > 1) {
+#pragma unroll
+      for (int r = 1; r < kRuns; ++r) {
+        sum = add2(sum, sh.before[r * LPR + w.lane]);
+        b = apply_map(b, sh.run[r * LPR + w.lane]);
+      }
+      if (!lost && !trade_maps<LPR, THREADS>(sh, step, run_map(sum, b), w, p)) {
+        lost = true;
+        if (p.status != nullptr) atomicOr(p.status, 1);
+      }
+      float2 before = c;
+      for (int r = 0; r < w.ranks; ++r) {
+        const float4 f = sh.factor[step & 1][r][w.lane];
+        RunMap m;
+        m.hi = make_float2(f.x, f.y);
+        m.lo = make_float2(f.z, f.w);
+        m.b = sh.b[step & 1][r][w.lane];
+        if (r == w.rank) before = c;
+        c = apply_map(c, m);
+      }
+      if (lost) c = before = make_float2(NAN, NAN);
+      carry = c;
+      c = before;
+    }
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      sh.before[r * LPR + w.lane] = c;
+      c = apply_map(c, sh.run[r * LPR + w.lane]);
+    }
+    if (w.ranks == 1) carry = c;
+  }
+  __syncthreads();
+  return sh.before[w.run * LPR + w.lane];
+}
+
+template <bool PAIR, int LPR, int THREADS>
+__device__ __forceinline__ void take_place(const RecurrenceParams& p, RecurrenceShared<LPR, THREADS>& sh, Team* team, Place* w) {
+  cg::cluster_group cluster = cg::this_cluster();
+  team->lane = threadIdx.x % LPR;
+  team->run = threadIdx.x / LPR;
+  team->ranks = cluster.num_blocks();
+  team->rank = cluster.block_rank();
+  *w = place<PAIR, LPR>(p, blockIdx.x / team->ranks, team->lane);
+  if (threadIdx.x == 0 && team->ranks > 1) {
+    for (int i = 0; i < 2; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&sh.arrived[i])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+}
+
+// Keeps the compiler from carrying what it derived from a value (decays, offsets) from one loop to the next: it has them
+// all in registers then, and those in memory.
+__device__ __forceinline__ void anew(uint32_t& v) { asm volatile("" : "+r"(v)); }
+__device__ __forceinline__ void anew(float2& v) { asm volatile("" : "+f"(v.x), "+f"(v.y)); }
+template <typename R, int T>
+__device__ __forceinline__ void anew(R (&v)[T]) {
+#pragma unroll
+  for (int t = 0; t < T; ++t) anew(v[t]);
+}
+
+__device__ __forceinline__ void load_after(uint32_t& r, const char* q, float after) {
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(q), "f"(after));
+}
+__device__ __forceinline__ void load_after(float2& r, const char* q, float after) {
+  asm volatile("ld.global.nc.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "l"(q), "f"(after));
+}
+__device__ __forceinline__ void load_after(uint16_t& r, const char* q, float after) {
+  asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(r) : "l"(q), "f"(after));
+}
+__device__ __forceinline__ void load_after(float& r, const char* q, float after) {
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(r) : "l"(q), "f"(after));
+}
+
+// A thread's two columns of the rows of a step: the rows' base is the same for the CTA, offsets inside a step fit 32 bits
+// (checked on the host). Columns past the last read the first one's and are not written.
+template <typename T, bool PAIR>
+struct Rows {
+  char* base;  // of the batch entry and head
+  uint32_t at, gap, row;  // bytes
+
+  __device__ __forceinline__ Rows(const RecurrenceTensor& t, const Place& w, int first) {
+    base = static_cast<char*>(t.ptr) + (w.b * t.sb + w.h * t.sh) * static_cast<long long>(sizeof(T));
+    row = static_cast<uint32_t>(t.sn) * sizeof(T);
+    at = (w.ok0 ? w.c0 * sizeof(T) : 0u) + first * row;
+    gap = w.ok1 ? w.gap * sizeof(T) : 0u;
+  }
+  __device__ __forceinline__ char* step(const RecurrenceTensor& t, long long token) const {
+    return base + token * t.sn * static_cast<long long>(sizeof(T));
+  }
+  // `after`: the load is issued behind what this value comes from, whose operands' registers it can take.
+  __device__ __forceinline__ typename PairOf<T>::Raw load(const char* step, uint32_t token, float after) const {
+    const char* q = step + (at + token * row);
+    typename PairOf<T>::Raw r;
+    if (PAIR) {
+      load_after(r, q, after);
+      return r;
+    }
+    typename PairOf<T>::Element a, b;
+    load_after(a, q, after);
+    load_after(b, q + gap, after);
+    return join_pair(a, b);
+  }
+  __device__ __forceinline__ void store(char* step, uint32_t token, const Place& w, float2 v) const {
+    store_pair<T, PAIR>(reinterpret_cast<T*>(step + (at + token * row)), w.gap, w.ok0, w.ok1, v);
+  }
+};
+
+// Runs with a gate of minus infinity, of which there are few, are summed out of line and from memory: in line their
+// second copy of the loops cost the kernels 50 registers.
+template <typename TX, typename TG, int T>
+__device__ __noinline__ float2 advance_from(float2 h, const typename PairOf<TX>::Raw* x, const typename PairOf<TG>::Raw* g,
+                                            float2* before) {
+#pragma unroll 1
+  for (int t = 0; t < T; ++t) {
+    if (before != nullptr) before[t] = h;
+    h = advance<TX, true>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+  }
+  return h;
+}
+template <typename TX, typename TG, int T>
+__device__ __noinline__ float2 retreat_from_zero(const typename PairOf<TX>::Raw* y, const typename PairOf<TG>::Raw* g) {
+  float2 r = make_float2(0.f, 0.f);
+#pragma unroll 1
+  for (int t = T - 1; t >= 0; --t) r = retreat<TX, true>(unpack_pair<TG>(g[t]), add2(unpack_pair<TX>(y[t]), r));
+  return r;
+}
+template <typename R, int T>
+struct InMemory {
+  R v[T];
+  __device__ __forceinline__ explicit InMemory(const R (&from)[T]) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) v[t] = from[t];
+  }
+};
+
+template <typename TX, typename TG, bool PAIR, int LPR, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_fwd_kernel(const RecurrenceParams p) {
+  constexpr int T = kRunTokens<TX, TG>;
+  __shared__ RecurrenceShared<LPR, THREADS> sh;
+  Team team;
+  Place w;
+  take_place<PAIR>(p, sh, &team, &w);
+  bool lost = false;
+  const int first = (team.rank * (THREADS / LPR) + team.run) * T;  // of the step's tokens
+  Rows<TX, PAIR> xr(p.x, w, first), orow(p.o, w, first);
+  Rows<TG, PAIR> gr(p.g, w, first);
+  const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
+  float2 carry = make_float2(0.f, 0.f);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
+
+  const int span = team.ranks * (THREADS / LPR) * T;  // tokens a step
+  const int steps = (p.n - 1) / span + 1, runs_all = (p.n - 1) / T + 1;
+  typename PairOf<TX>::Raw x[T];
+  typename PairOf<TG>::Raw g[T];
+  auto fetch = [&](int t, int step, float after) {  // one token of the step; none behind the last: the identity
+    zero_pair(x[t]);
+    zero_pair(g[t]);
+    if (step * span + first + t < p.n) {
+      x[t] = xr.load(xr.step(p.x, static_cast<long long>(step) * span), t, after);
+      g[t] = gr.load(gr.step(p.g, static_cast<long long>(step) * span), t, after);
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < T; ++t) fetch(t, 0, 0.f);
+  if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
+  for (int step = 0; step < steps; ++step) {
+    const int t0 = step * span + first;
+    float2 sum = make_float2(0.f, 0.f), h = sum;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float2 gv = unpack_pair<TG>(g[t]);
+      sum = add2(sum, gv);
+      h = advance<TX, false>(gv, h, unpack_pair<TX>(x[t]));
+    }
+    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    if (drops) {
+      const InMemory<typename PairOf<TX>::Raw, T> xm(x);
+      const InMemory<typename PairOf<TG>::Raw, T> gm(g);
+      h = advance_from<TX, TG, T>(make_float2(0.f, 0.f), xm.v, gm.v, nullptr);
+    }
+    h = exchange(sh, step, sum, h, team, p, carry, lost);
+    if (p.states != nullptr && t0 < p.n)
+      store_pair<float, PAIR>(p.states + state_of(p, w, t0 / T, runs_all), w.gap, w.ok0, w.ok1, h);
+    char* os = orow.step(p.o, static_cast<long long>(step) * span);
+    anew(x);
+    anew(g);
+    anew(xr.row);
+    anew(gr.row);
+    anew(orow.row);
+    if (!drops && (step + 2) * span <= p.n) {  // this step and the next are whole
+      const char* xs = xr.step(p.x, static_cast<long long>(step + 1) * span);
+      const char* gs = gr.step(p.g, static_cast<long long>(step + 1) * span);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+        orow.store(os, t, w, h);
+        x[t] = xr.load(xs, t, h.x);  // the next step's, as soon as its place is free
+        g[t] = gr.load(gs, t, h.x);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        h = advance<TX, true>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+        if (t0 + t < p.n) orow.store(os, t, w, h);
+        fetch(t, step + 1, h.x);
+      }
+    }
+  }
+  if (p.end != nullptr && team.run == 0 && team.rank == 0)
+    store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
+  if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
+}
+
+template <typename TX, typename TG, bool PAIR, int LPR, int THREADS>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_kernel(const RecurrenceParams p) {
+  constexpr int T = kRunTokens<TX, TG>;
+  __shared__ RecurrenceShared<LPR, THREADS> sh;
+  Team team;
+  Place w;
+  take_place<PAIR>(p, sh, &team, &w);
+  bool lost = false;
+  const int span = team.ranks * (THREADS / LPR);                        // runs a step
+  const int nth = span - 1 - (team.rank * (THREADS / LPR) + team.run);  // of the step's runs, in the order of the tokens
+  const int first = nth * T;
+  Rows<TX, PAIR> xr(p.x, w, first), yr(p.o, w, first), dxr(p.dx, w, first);
+  Rows<TG, PAIR> gr(p.g, w, first), dgr(p.dg, w, first);
+  const bool has_dy = p.o.ptr != nullptr, want_dx = p.dx.ptr != nullptr, want_dg = p.dg.ptr != nullptr;
+  const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
+  float2 carry = make_float2(0.f, 0.f);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
+
+  const int runs_all = (p.n - 1) / T + 1;
+  const int steps = (runs_all - 1) / span + 1;
+  typename PairOf<TX>::Raw x[T], y[T];
+  typename PairOf<TG>::Raw g[T];
+  float2 state;
+  auto rows_x = [&](int t, int step, float after) {
+    zero_pair(x[t]);
+    if (step * span * T + first + t < p.n) x[t] = xr.load(xr.step(p.x, static_cast<long long>(step) * span * T), t, after);
+  };
+  auto rows_gy = [&](int t, int step, float after) {
+    zero_pair(g[t]);
+    zero_pair(y[t]);
+    if (step * span * T + first + t < p.n) {
+      g[t] = gr.load(gr.step(p.g, static_cast<long long>(step) * span * T), t, after);
+      if (has_dy) y[t] = yr.load(yr.step(p.o, static_cast<long long>(step) * span * T), t, after);
+    }
+  };
+  auto load_state = [&](int step) {
+    state = make_float2(0.f, 0.f);
+    const int run = step * span + nth;
+    if (run < runs_all) state = load_pair<float, PAIR>(p.states + state_of(p, w, run, runs_all), w.gap, w.ok0, w.ok1);
+  };
+  load_state(steps - 1);
+#pragma unroll
+  for (int t = 0; t < T; ++t) rows_x(t, steps - 1, 0.f);
+#pragma unroll
+  for (int t = T - 1; t >= 0; --t) rows_gy(t, steps - 1, 0.f);
+  if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
+  // The walk starts at the end; the runs behind the last token are the identity. Steps before the last one are whole.
+  for (int step = steps - 1; step >= 0; --step) {
+    float2 sum = make_float2(0.f, 0.f), r = sum, h = state;
+#pragma unroll
+    for (int t = T - 1; t >= 0; --t) {
+      const float2 gv = unpack_pair<TG>(g[t]);
+      sum = add2(sum, gv);
+      r = retreat<TX, false>(gv, add2(unpack_pair<TX>(y[t]), r));
+    }
+    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    float2 before[T];  // the state before each token
+    anew(g);
+    if (drops) {
+      const InMemory<typename PairOf<TX>::Raw, T> xm(x), ym(y);
+      const InMemory<typename PairOf<TG>::Raw, T> gm(g);
+      float2 bm[T];
+      r = retreat_from_zero<TX, TG, T>(ym.v, gm.v);
+      advance_from<TX, TG, T>(h, xm.v, gm.v, bm);
+#pragma unroll
+      for (int t = 0; t < T; ++t) before[t] = bm[t];
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        before[t] = h;
+        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+      }
+    }
+    anew(y);
+    anew(g);
+    anew(xr.row);
+    if (step > 0) {  // x and the state are done with: the next step's
+      load_state(step - 1);
+      const char* xs = xr.step(p.x, static_cast<long long>(step - 1) * span * T);
+#pragma unroll
+      for (int t = 0; t < T; ++t) x[t] = xr.load(xs, t, before[t].x);
+    }
+    r = exchange(sh, steps - 1 - step, sum, r, team, p, carry, lost);
+    const long long token = static_cast<long long>(step) * span * T;
+    anew(yr.row);
+    anew(gr.row);
+    anew(dxr.row);
+    anew(dgr.row);
+    char *dxs = dxr.step(p.dx, token), *dgs = dgr.step(p.dg, token);
+    if (!drops && step > 0 && step < steps - 1 && has_dy && want_dx && want_dg) {
+      const char *ys = yr.step(p.o, token - static_cast<long long>(span) * T), *gs = gr.step(p.g, token - static_cast<long long>(span) * T);
+#pragma unroll
+      for (int t = T - 1; t >= 0; --t) {
+        const float2 all = add2(unpack_pair<TX>(y[t]), r);
+        dxr.store(dxs, t, w, all);
+        r = retreat<TX, false>(unpack_pair<TG>(g[t]), all);
+        dgr.store(dgs, t, w, mul2(r, before[t]));
+        y[t] = yr.load(ys, t, r.x);
+        g[t] = gr.load(gs, t, r.x);
+      }
+    } else {
+#pragma unroll
+      for (int t = T - 1; t >= 0; --t) {
+        const float2 gv = unpack_pair<TG>(g[t]), all = add2(unpack_pair<TX>(y[t]), r);
+        const bool in = token + first + t < p.n;
+        if (in && want_dx) dxr.store(dxs, t, w, all);
+        r = retreat<TX, true>(gv, all);
+        if (in && want_dg) {
+          float2 d = mul2(r, before[t]);
+          if (gv.x == -INFINITY) d.x = 0.f;
+          if (gv.y == -INFINITY) d.y = 0.f;
+          dgr.store(dgs, t, w, d);
+        }
+        if (step > 0) rows_gy(t, step - 1, r.x);
+      }
+    }
+  }
+  if (p.end != nullptr && team.run == 0 && team.rank == 0)
+    store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
+  if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
 }
 
 }  // namespace fla
@@ -375,7 +697,7 @@ namespace {
 using fla::RecurrenceParams;
 using fla::RecurrenceTensor;
 
-constexpr int kAloneTokens = 32;  // sequences up to here have nothing to exchange
+constexpr int kShortTokens = 32;  // sequences up to here have nothing to exchange
 
 int element_bytes(int dtype) { return dtype == FLA_DTYPE_F32 ? 4 : 2; }
 
@@ -386,6 +708,7 @@ struct Plan {
   bool pair;
   int lpr;
   int batch;
+  long long farthest;  // bytes from one token to the next, of the tensor where they are most
 };
 
 void add_tensor(const FlaTensor& t, RecurrenceTensor* out) {
@@ -408,6 +731,9 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
   p.start = backward ? a->r_init : a->s_init;
   p.end = backward ? a->r_final : a->s_final;
   p.states = static_cast<float*>(a->states);
+  p.status = a->status;
+  p.wait_limit_ns = (a->wait_limit_us ? a->wait_limit_us : 2000000ull) * 1000ull;
+  p.withhold = (a->debug_flags & FLA_DEBUG_WITHHOLD_FIRST_TILE) != 0;
   p.heads = a->heads;
   p.n = a->seqlen;
   p.c = a->dim;
@@ -418,7 +744,7 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
   auto every = [&](auto&& holds) {
     bool ok = true;
     for (int i = 0; i < 5; ++i)
-      if (all[i]->ptr != nullptr) ok = ok && holds(*all[i], sizes[i]);
+      if (all[i]->ptr != nullptr) ok = holds(*all[i], sizes[i]) && ok;
     return ok;
   };
   const long long wide = static_cast<long long>(p.heads) * p.c;
@@ -438,65 +764,70 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
                 return reinterpret_cast<uintptr_t>(t.ptr) % (2 * size) == 0 && (p.n == 1 || t.sn % 2 == 0) &&
                        (p.heads == 1 || t.sh % 2 == 0) && (plan.batch == 1 || t.sb % 2 == 0);
               });
+  plan.farthest = 1;
+  every([&](const RecurrenceTensor& t, int size) {
+    plan.farthest = std::max(plan.farthest, t.sn * size);
+    return true;
+  });
   plan.lpr = p.c <= 32 ? 16 : 32;
   p.tiles = (p.c + 2 * plan.lpr - 1) / (2 * plan.lpr);
   p.tiles_all = static_cast<long long>(p.tiles) * p.heads * plan.batch;
   return plan;
 }
 
-// CTAs of a cluster and threads of a CTA. A tile of channels is walked by one cluster from end to end; more CTAs walk
-// it in fewer steps. Two CTAs are resident an SM.
-void shape_of(const Plan& plan, int run_tokens, int sm_count, int* threads, int* ranks) {
+// CTAs of a cluster and threads of a CTA. A tile of channels is walked by one cluster from end to end; more CTAs, and
+// larger ones, walk it in fewer steps.
+struct Shape {
+  int threads, ranks;
+};
+Shape shape_of(const Plan& plan, int run_tokens, int most_threads, int sm_count) {
   const long long runs = (plan.p.n - 1) / run_tokens + 1;
-  int per_cta = 1;
-  while (per_cta < fla::kRecThreads / plan.lpr && per_cta < runs) per_cta *= 2;
-  int r = 1;
-  while (r < fla::kRecMaxCluster && plan.p.tiles_all * r < 2 * sm_count && static_cast<long long>(r) * per_cta < runs) r *= 2;
-  *threads = std::max(32, per_cta * plan.lpr);
-  *ranks = r;
+  Shape s = {256, 1};
+  auto step = [&] { return static_cast<long long>(s.ranks) * s.threads / plan.lpr; };
+  while (s.ranks < fla::kRecMaxCluster && plan.p.tiles_all * s.ranks < 2 * sm_count && step() < runs) s.ranks *= 2;
+  if (plan.p.tiles_all * s.ranks <= sm_count && step() < runs) s.threads = most_threads;
+  return s;
 }
 
-template <typename TX, typename TG, bool PAIR, int LPR, bool ALONE>
+template <typename TX, typename TG, bool PAIR, int LPR>
 int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
-  int threads = 128, ranks = 1;
-  long long blocks;
-  if (ALONE) {
-    blocks = (plan.p.tiles_all * LPR + threads - 1) / threads;
-  } else {
-    shape_of(plan, fla::kRunTokens<TX, TG>, sm_count, &threads, &ranks);
-    blocks = plan.p.tiles_all * ranks;
+  constexpr int T = fla::kRunTokens<TX, TG>;
+  Shape shape = shape_of(plan, T, backward ? 512 : 1024, sm_count);
+  const bool alone = plan.p.n <= kShortTokens || plan.farthest > 0x7fffffffLL / (shape.ranks * (shape.threads / LPR) * T);
+  long long blocks = plan.p.tiles_all * shape.ranks;
+  if (alone) {
+    shape = {fla::kShortThreads, 1};
+    blocks = (plan.p.tiles_all * LPR + shape.threads - 1) / shape.threads;
   }
   if (blocks > 0x7fffffffLL) return FLA_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(shape.threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.x = shape.ranks;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
-  if (backward)
-    return fla::launched(cudaLaunchKernelEx(&cfg, fla::fla_recurrence_bwd_kernel<TX, TG, PAIR, LPR, ALONE>, plan.p),
-                         "fla_recurrence_bwd_kernel");
-  return fla::launched(cudaLaunchKernelEx(&cfg, fla::fla_recurrence_fwd_kernel<TX, TG, PAIR, LPR, ALONE>, plan.p),
-                       "fla_recurrence_fwd_kernel");
+  cfg.numAttrs = shape.ranks > 1 ? 1 : 0;
+  auto go = [&](auto kernel, const char* name) { return fla::launched(cudaLaunchKernelEx(&cfg, kernel, plan.p), name); };
+  if (alone)
+    return backward ? go(fla::fla_recurrence_short_bwd_kernel<TX, TG, PAIR, LPR>, "fla_recurrence_short_bwd_kernel")
+                    : go(fla::fla_recurrence_short_fwd_kernel<TX, TG, PAIR, LPR>, "fla_recurrence_short_fwd_kernel");
+  if (shape.threads == 256)
+    return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_bwd_kernel")
+                    : go(fla::fla_recurrence_fwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_fwd_kernel");
+  return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, PAIR, LPR, 512>, "fla_recurrence_bwd_kernel")
+                  : go(fla::fla_recurrence_fwd_kernel<TX, TG, PAIR, LPR, 1024>, "fla_recurrence_fwd_kernel");
 }
 
 template <typename TX, typename TG>
 int launch_types(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
-  const bool alone = plan.p.n <= kAloneTokens;
-  auto pick = [&](auto pair, auto lpr) {
-    constexpr bool P = decltype(pair)::value;
-    constexpr int L = decltype(lpr)::value;
-    return alone ? launch<TX, TG, P, L, true>(plan, backward, sm_count, stream)
-                 : launch<TX, TG, P, L, false>(plan, backward, sm_count, stream);
-  };
-  using L16 = std::integral_constant<int, 16>;
-  using L32 = std::integral_constant<int, 32>;
-  if (plan.pair) return plan.lpr == 16 ? pick(std::true_type(), L16()) : pick(std::true_type(), L32());
-  return plan.lpr == 16 ? pick(std::false_type(), L16()) : pick(std::false_type(), L32());
+  if (plan.pair)
+    return plan.lpr == 16 ? launch<TX, TG, true, 16>(plan, backward, sm_count, stream)
+                          : launch<TX, TG, true, 32>(plan, backward, sm_count, stream);
+  return plan.lpr == 16 ? launch<TX, TG, false, 16>(plan, backward, sm_count, stream)
+                        : launch<TX, TG, false, 32>(plan, backward, sm_count, stream);
 }
 
 bool known_type(int t) { return t == FLA_DTYPE_BF16 || t == FLA_DTYPE_F16 || t == FLA_DTYPE_F32; }

@@ -5,11 +5,12 @@ state before and behind them. The reference has no counterpart.
 from __future__ import annotations
 
 import ctypes
+import os
 from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._lib import FlaRecurrenceArgs
 from .ops import _desc
 
@@ -77,9 +78,16 @@ def _args(x: torch.Tensor, g: torch.Tensor) -> FlaRecurrenceArgs:
 def _call(name: str, a: FlaRecurrenceArgs, device: torch.device) -> None:
     with torch.cuda.device(device):
         a.stream = torch.cuda.current_stream(device).cuda_stream
+        a.status, a.debug_flags = ops._status_word(device).data_ptr(), ops._debug_flags
         rc = getattr(_lib.load(), name)(ctypes.byref(a))
     if rc != 0:
         raise RuntimeError(f"flashlinear: {name} returned {rc}: {_lib.strerror(rc)}")
+    _debug_check(device)
+
+
+def _debug_check(device: torch.device) -> None:
+    if os.environ.get("FLA_DEBUG", "0") == "1":
+        ops.check_status(device)
 
 
 def recurrence_fwd(
@@ -89,8 +97,9 @@ def recurrence_fwd(
     token, and, with keep_states, what recurrence_bwd needs of the pass (a byte buffer private to the library)."""
     native = _lib.host() if x.is_cuda else None
     if native is not None:
-        res = native.recurrence_forward(x, log_decay, s_init, keep_states)
+        res = native.recurrence_forward(x, log_decay, s_init, keep_states, ops._debug_flags, ops._status_ptr(x))
         if res is not None:
+            _debug_check(x.device)
             return res
     check_inputs(x, log_decay, s_init)
     B, H, N, D = x.shape
@@ -125,8 +134,9 @@ def recurrence_bwd(
     back here. None for a gradient of the outputs is zero; `needs` says which results are wanted (the others are None)."""
     native = _lib.host() if x.is_cuda else None
     if native is not None:
-        res = native.recurrence_backward(grad_out, x, log_decay, states, grad_s_final, *needs)
+        res = native.recurrence_backward(grad_out, x, log_decay, states, grad_s_final, *needs, ops._debug_flags, ops._status_ptr(x))
         if res is not None:
+            _debug_check(x.device)
             return res
     check_inputs(x, log_decay, grad_s_final)
     B, H, N, D = x.shape

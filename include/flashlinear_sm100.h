@@ -353,7 +353,9 @@ int fla_sm100_taylor_bwd(const FlaArgs* args);
  * few tokens, of recurrence_states_bytes(), 16-byte aligned, private to the library, for the backward of the same x and g.
  * bwd reads x, g, d_o (null: zero), r_init (gradient of s_final, null: zero) and `states`, writes d_x, d_g and
  * r_final (gradient of s_init), each unless null. Gates must not make the state overflow fp32 within a sequence.
- * No scratch; one launch; sums in an order that depends on the shapes and strides only. */
+ * No scratch; one launch; sums in an order that depends on the shapes and strides only. The CTAs of a cluster wait for each
+ * other's sums, with the limit of FlaArgs::wait_limit_us; one that runs out sets bit 0 of *status (optional) and fills what
+ * it could not compute with NaN. debug_flags: FLA_DEBUG_WITHHOLD_FIRST_TILE makes that happen, for a test. */
 typedef struct FlaRecurrenceArgs {
   int32_t batch, heads, seqlen, dim;
   int32_t dtype, g_dtype;
@@ -366,7 +368,10 @@ typedef struct FlaRecurrenceArgs {
   float* r_final;
   void* states;
   size_t states_bytes;
+  int32_t* status;
   void* stream;
+  uint32_t wait_limit_us;
+  uint32_t debug_flags;
 } FlaRecurrenceArgs;
 size_t fla_sm100_recurrence_states_bytes(const FlaRecurrenceArgs* args);
 int fla_sm100_recurrence_fwd(const FlaRecurrenceArgs* args);

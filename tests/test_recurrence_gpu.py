@@ -169,6 +169,29 @@ def test_nothing_passes_a_reset(poison, N):
         assert torch.equal(got["out"][:, :, at:], clean["out"][:, :, at:])
 
 
+def test_a_wait_that_runs_out():
+    """A peer whose sums never come: the wait ends at its limit, bit 0 of the status is set, what hangs on it is NaN,
+    and the next call is right again. (The limit is that of the call; nothing is left waiting.)"""
+    import ctypes
+
+    from flashy_linear_attention_b200 import _lib, ops, recurrence as rec
+
+    x, g, s, _, _ = make(1, 1, 5000, 64)
+    ops.check_status(x.device)
+    out, s_final = torch.zeros_like(x), torch.zeros(1, 1, 64, device=DEV)
+    a = rec._args(x, g)
+    a.o, a.s_init, a.s_final = rec._desc(out), s.data_ptr(), s_final.data_ptr()
+    a.status, a.stream = ops._status_word(x.device).data_ptr(), torch.cuda.current_stream().cuda_stream
+    a.wait_limit_us, a.debug_flags = 20000, _lib.FLA_DEBUG_WITHHOLD_FIRST_TILE
+    assert _lib.load().fla_sm100_recurrence_fwd(ctypes.byref(a)) == 0
+    with pytest.raises(RuntimeError, match="status 1"):
+        ops.check_status(x.device)
+    assert out.isnan().any() and s_final.isnan().all()
+    got = recurrence().apply(x, g, s)
+    ops.check_status(x.device)
+    check("out", got[0], reference(x, g, s)["out"])
+
+
 @pytest.mark.parametrize("N", [20, 700])
 def test_an_infinity_stays_until_it_is_dropped(N):
     x, g, s, _, _ = make(1, 1, N, 64, reset=0.0, rate=(1e-3, 8.0))
