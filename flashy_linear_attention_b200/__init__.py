@@ -7,10 +7,13 @@ flashlinear/kernels/__init__.py:1-5):
     linear_flash_wrapper_fwd_smallv_hd, linear_flash_wrapper_bwd_smallv_hd
 plus the lower-level causal_dot_product_fwd / causal_dot_product_bwd (running-state arguments),
 LinearAttentionResumable (state carried across calls), LinearAttentionNormalized (the README's
-denominator fused into streaming kernels) and host.HostPipeline (pinned host tensors).
+denominator fused into streaming kernels), host.HostPipeline (pinned host tensors), and what stands beside an
+attention in a block: GatedLinearRecurrence, LayerNorm and AddLayerNorm.
 """
 from .functions import (
+    AddLayerNorm,
     GatedLinearRecurrence,
+    LayerNorm,
     LinearAttention,
     LinearAttentionNormalized,
     LinearAttentionResumable,
@@ -35,6 +38,8 @@ __all__ = [
     "LinearAttentionNormalized",
     "TaylorLinearAttention",
     "GatedLinearRecurrence",
+    "LayerNorm",
+    "AddLayerNorm",
     "linear_flash_wrapper_fwd",
     "linear_flash_wrapper_bwd",
     "linear_flash_wrapper_fwd_smallv_hd",

@@ -93,6 +93,34 @@ class FlaRecurrenceArgs(ctypes.Structure):
     ]
 
 
+class FlaLayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("w_dtype", ctypes.c_int32),
+        ("per_head", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("x", FlaTensor),
+        ("residual", FlaTensor),
+        ("sum", FlaTensor),
+        ("y", FlaTensor),
+        ("d_y", FlaTensor),
+        ("d_sum", FlaTensor),
+        ("d_x", FlaTensor),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("d_weight", ctypes.c_void_p),
+        ("d_bias", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 class FlaExchange(ctypes.Structure):
     _fields_ = [
         ("rank", ctypes.c_int32),
@@ -151,6 +179,9 @@ EXPORTED_SYMBOLS = (
     "fla_sm100_recurrence_states_bytes",
     "fla_sm100_recurrence_fwd",
     "fla_sm100_recurrence_bwd",
+    "fla_sm100_layer_norm_workspace_bytes",
+    "fla_sm100_layer_norm_fwd",
+    "fla_sm100_layer_norm_bwd",
 )
 
 _lib = None
@@ -248,6 +279,9 @@ def load() -> ctypes.CDLL:
     lib.fla_sm100_state_exchange.restype = ctypes.c_int
     lib.fla_sm100_state_exchange.argtypes = [ctypes.POINTER(FlaArgs), ctypes.c_int, ctypes.POINTER(FlaExchange)]
     lib.fla_sm100_last_launch_count.restype = ctypes.c_int
+    lib.fla_sm100_layer_norm_workspace_bytes.restype = ctypes.c_size_t
+    for name in ("fla_sm100_layer_norm_workspace_bytes", "fla_sm100_layer_norm_fwd", "fla_sm100_layer_norm_bwd"):
+        getattr(lib, name).argtypes = [ctypes.POINTER(FlaLayerNormArgs)]
     lib.fla_sm100_recurrence_states_bytes.restype = ctypes.c_size_t
     for name in ("fla_sm100_recurrence_states_bytes", "fla_sm100_recurrence_fwd", "fla_sm100_recurrence_bwd"):
         getattr(lib, name).argtypes = [ctypes.POINTER(FlaRecurrenceArgs)]

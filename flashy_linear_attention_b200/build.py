@@ -20,7 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libflashlinear_sm100.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
-SOURCES = ["fla_api.cu", "fla_recurrence.cu"]
+SOURCES = ["fla_api.cu", "fla_recurrence.cu", "fla_layer_norm.cu"]
 HOST_SOURCES = ["fla_host.cpp", os.path.join("..", "..", "include", "flashlinear_sm100.h")]
 HEADERS = ["fla_kernel.cuh", "fla_backward.cuh", "fla_wide_kernel.cuh", "fla_normalize.cuh", "fla_taylor.cuh", "fla_taylor_attention.cuh", "fla_decode.cuh", "fla_internal.h", "fla_pairs.cuh", "ptx.cuh", os.path.join("..", "..", "include", "flashlinear_sm100.h")]
 

@@ -490,6 +490,104 @@ std::optional<std::array<OptTensor, 3>> recurrence_backward(const OptTensor& dy,
   return out;
 }
 
+// Layer norm, of rows in up to four dimensions.
+bool norm_rows(const Tensor& t, const Tensor& x) {
+  return t.layout() == at::kStrided && t.dim() >= 1 && t.dim() <= 4 && t.is_cuda() && t.device() == x.device() && !t.is_neg() &&
+         t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && (t.stride(-1) == 1 || t.size(-1) == 1);
+}
+bool norm_weights(const OptTensor& w, const Tensor& x) {
+  if (!w.has_value()) return true;
+  if (!w->is_cuda() || w->device() != x.device() || !w->is_contiguous() || w->is_neg() || w->size(-1) != x.size(-1)) return false;
+  if (w->dim() != 1 && !(w->dim() == 2 && x.dim() == 4 && w->size(0) == x.size(1))) return false;
+  return float_type(*w) == float_type(x) || float_type(*w) == FLA_DTYPE_F32;
+}
+bool norm_covered(const Tensor& x, const OptTensor& w, const OptTensor& b) {
+  if (!norm_rows(x, x) || float_type(x) < 0 || x.numel() == 0 || x.size(-1) > 32768 || x.numel() / x.size(-1) > INT32_MAX)
+    return false;
+  if (!norm_weights(w, x) || !norm_weights(b, x)) return false;
+  return !w.has_value() || !b.has_value() || (w->sizes() == b->sizes() && w->scalar_type() == b->scalar_type());
+}
+FlaTensor norm_desc(const Tensor& t) {  // [B, H, N, D], [B, N, D], [N, D] or [D]
+  const int64_t n = t.dim();
+  FlaTensor d = {};
+  d.ptr = t.data_ptr();
+  if (n >= 2) d.stride_n = t.stride(n - 2);
+  if (n == 4) d.stride_h = t.stride(1);
+  if (n >= 3) d.stride_b = t.stride(0);
+  return d;
+}
+Tensor norm_like(const Tensor& t) {
+  const Tensor out = at::empty_like(t);
+  return norm_rows(out, t) ? out : at::empty(t.sizes(), t.options());
+}
+FlaLayerNormArgs norm_args(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  const int64_t n = x.dim();
+  FlaLayerNormArgs a = {};
+  a.batch = n >= 3 ? static_cast<int32_t>(x.size(0)) : 1;
+  a.heads = n == 4 ? static_cast<int32_t>(x.size(1)) : 1;
+  a.tokens = n >= 2 ? static_cast<int32_t>(x.size(n - 2)) : 1;
+  a.dim = static_cast<int32_t>(x.size(n - 1));
+  a.dtype = a.w_dtype = float_type(x);
+  for (const OptTensor* t : {&w, &b})
+    if (t->has_value()) {
+      a.w_dtype = float_type(**t);
+      a.per_head = (*t)->dim() == 2;
+    }
+  a.eps = static_cast<float>(eps);
+  a.x = norm_desc(x);
+  if (w.has_value()) a.weight = w->data_ptr();
+  if (b.has_value()) a.bias = b->data_ptr();
+  a.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+  return a;
+}
+struct Norm {
+  Tensor out;
+  OptTensor sum, stats;
+};
+std::optional<Norm> layer_norm_forward(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps,
+                                       const OptTensor& residual, bool keep_stats) {
+  if (!norm_covered(x, w, b) || (residual.has_value() && !norm_rows(*residual, x)) || !(eps >= 0)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  FlaLayerNormArgs a = norm_args(x, w, b, eps);
+  Norm r{norm_like(x), std::nullopt, std::nullopt};
+  a.y = norm_desc(r.out);
+  if (residual.has_value()) {
+    r.sum = norm_like(x);
+    a.residual = norm_desc(*residual);
+    a.sum = norm_desc(*r.sum);
+  }
+  if (keep_stats) {
+    r.stats = at::empty({x.numel() / x.size(-1), 2}, x.options().dtype(at::kFloat));
+    a.stats = r.stats->data_ptr<float>();
+  }
+  check(fla_sm100_layer_norm_fwd(&a), "fla_sm100_layer_norm_fwd");
+  return r;
+}
+std::optional<std::array<OptTensor, 3>> layer_norm_backward(const Tensor& dy, const Tensor& x, const OptTensor& w, const OptTensor& b,
+                                                            const Tensor& stats, const OptTensor& ds, bool need_x, bool need_w,
+                                                            bool need_b) {
+  if (!norm_covered(x, w, b) || !norm_rows(dy, x) || (ds.has_value() && !norm_rows(*ds, x)) || !stats.is_cuda() ||
+      stats.scalar_type() != at::kFloat || !stats.is_contiguous() || !(need_x || need_w || need_b))
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  FlaLayerNormArgs a = norm_args(x, w, b, 0.0);
+  a.d_y = norm_desc(dy);
+  if (ds.has_value()) a.d_sum = norm_desc(*ds);
+  a.stats = stats.data_ptr<float>();
+  std::array<OptTensor, 3> out;
+  if (need_x) a.d_x = norm_desc(*(out[0] = norm_like(x)));
+  if (need_w) a.d_weight = (out[1] = at::empty(w->sizes(), w->options()))->data_ptr();
+  if (need_b) a.d_bias = (out[2] = at::empty(b->sizes(), b->options()))->data_ptr();
+  Tensor ws;
+  if (const size_t need = fla_sm100_layer_norm_workspace_bytes(&a)) {
+    ws = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = need;
+  }
+  check(fla_sm100_layer_norm_bwd(&a), "fla_sm100_layer_norm_bwd");
+  return out;
+}
+
 // What is saved beside the repacked copy of an input that is not kept itself: an empty tensor that shares
 // its version count, for autograd to see that it was changed in place. (An inference tensor has none;
 // it is returned itself, and autograd refuses it as it always does.)
@@ -517,6 +615,26 @@ PYBIND11_MODULE(_hostcalls, m) {
     return py::make_tuple(r->out, r->s_final, r->seg_states, views);
   });
   m.def("version_of", &version_of);
+  m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, const OptTensor& residual,
+                                 bool keep_stats) -> py::object {
+    std::optional<Norm> r;
+    {
+      const py::gil_scoped_release unlocked;
+      r = layer_norm_forward(x, w, b, eps, residual, keep_stats);
+    }
+    if (!r.has_value()) return py::none();
+    return py::make_tuple(r->out, r->sum, r->stats);
+  });
+  m.def("layer_norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& w, const OptTensor& b, const Tensor& stats,
+                                  const OptTensor& ds, bool need_x, bool need_w, bool need_b) -> py::object {
+    std::optional<std::array<OptTensor, 3>> r;
+    {
+      const py::gil_scoped_release unlocked;
+      r = layer_norm_backward(dy, x, w, b, stats, ds, need_x, need_w, need_b);
+    }
+    if (!r.has_value()) return py::none();
+    return py::make_tuple((*r)[0], (*r)[1], (*r)[2]);
+  });
   m.def("recurrence_forward", [](const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep_states,
                                  unsigned debug_flags, uintptr_t status) -> py::object {
     std::optional<Recurrence> r;

@@ -15,7 +15,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import ops, recurrence
+from . import layer_norm, ops, recurrence
 
 
 def _autocast_to_bf16(forward):
@@ -279,3 +279,56 @@ class GatedLinearRecurrence(Function):
             return None, None, None
         needs = tuple(ctx.needs_input_grad) + (False,) * (3 - len(ctx.needs_input_grad))
         return tuple(recurrence.recurrence_bwd(grad_output, x, log_decay, states, grad_s_final, needs)[:len(ctx.needs_input_grad)])
+
+
+class LayerNorm(Function):
+    """Layer norm over the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``.
+
+    ``LayerNorm.apply(x, weight=None, bias=None, eps=1e-5)`` for x ``[..., D]`` of any rank and strides (bf16, fp16 or fp32, D
+    up to 32768); weight and bias ``[D]``, or for x ``[B, H, N, D]`` also ``[H, D]``: an affine map of each head's own, which
+    normalises an attention's unnormalised output head by head, the usual alternative to its denominator
+    (``LinearAttentionNormalized``). They have x's type or fp32, and so have their gradients, which are summed in fp32 over
+    all rows in a fixed order and rounded once. Autocast changes nothing: the result has x's type.
+
+    The reference has no counterpart.
+    """
+
+    @staticmethod
+    def forward(ctx: Any, x, weight=None, bias=None, eps: float = 1e-5):
+        out, _, stats = layer_norm.layer_norm_fwd(x, weight, bias, eps, None, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, stats)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_output):
+        needs = (tuple(ctx.needs_input_grad) + (False,) * 3)[:3]
+        grads = layer_norm.layer_norm_bwd(grad_output, *ctx.saved_tensors, None, needs)
+        return (*grads, None)[:len(ctx.needs_input_grad)]
+
+
+class AddLayerNorm(Function):
+    """Addition of a residual and layer norm in one pass: ``sum = x + residual`` (rounded to their type),
+    ``out = LayerNorm(sum)``.
+
+    ``out, sum = AddLayerNorm.apply(x, residual, weight=None, bias=None, eps=1e-5)``, shapes and types as for ``LayerNorm``.
+    ``sum`` is the residual of the next block, and its gradient joins that of ``out`` in one pass backward: x and the
+    residual get the same gradient. The reference has no counterpart.
+    """
+
+    @staticmethod
+    def forward(ctx: Any, x, residual, weight=None, bias=None, eps: float = 1e-5):
+        out, total, stats = layer_norm.layer_norm_fwd(x, weight, bias, eps, residual, any(ctx.needs_input_grad[:4]))
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(total, weight, bias, stats)
+        return out, total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_output, grad_sum):
+        count = len(ctx.needs_input_grad)
+        if grad_output is None:  # the sum alone was used
+            return (grad_sum, grad_sum, None, None, None)[:count]
+        needs = (tuple(ctx.needs_input_grad) + (False,) * 4)[:4]
+        dx, dw, db = layer_norm.layer_norm_bwd(grad_output, *ctx.saved_tensors, grad_sum, (needs[0] or needs[1], *needs[2:]))
+        return (dx, dx, dw, db, None)[:count]

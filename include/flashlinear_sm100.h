@@ -377,6 +377,37 @@ size_t fla_sm100_recurrence_states_bytes(const FlaRecurrenceArgs* args);
 int fla_sm100_recurrence_fwd(const FlaRecurrenceArgs* args);
 int fla_sm100_recurrence_bwd(const FlaRecurrenceArgs* args);
 
+/* ---- layer norm ----
+ * Rows of dim columns in [batch, heads, tokens, dim] tensors, any strides (zero included for inputs), innermost stride 1,
+ * nothing aligned beyond its element size (faster where all rows are 16-byte aligned and dim is a multiple of 16 bytes).
+ * dtype: of all rows; w_dtype: of weight, bias and their gradients, the same or fp32. weight and bias (each may be null)
+ * are [dim], or with per_head [heads, dim], contiguous. dim up to 32768, rows up to 2^31 - 1.
+ * fwd: y = (s - mean) / sqrt(var + eps) * weight + bias with s = x, or, where residual is given, s = x + residual rounded to
+ * dtype, which is written to sum. stats (optional, fp32 [2 * rows], 8-byte aligned, private to the library) is kept for:
+ * bwd: x is the s of the forward, d_y the gradient of y, d_sum (optional) that of sum; writes d_x (the gradient of x and of the
+ * residual), d_weight and d_bias, each unless null. Gradients of the weights are summed in fp32 in a fixed order; they take
+ * layer_norm_workspace_bytes() of scratch for the same arguments, 16-byte aligned, and a second launch. */
+typedef struct FlaLayerNormArgs {
+  int32_t batch, heads, tokens, dim;
+  int32_t dtype, w_dtype;
+  int32_t per_head;
+  float eps;
+  FlaTensor x, residual;
+  FlaTensor sum, y;
+  FlaTensor d_y, d_sum, d_x;
+  const void* weight;
+  const void* bias;
+  void* d_weight;
+  void* d_bias;
+  float* stats;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} FlaLayerNormArgs;
+size_t fla_sm100_layer_norm_workspace_bytes(const FlaLayerNormArgs* args);
+int fla_sm100_layer_norm_fwd(const FlaLayerNormArgs* args);
+int fla_sm100_layer_norm_bwd(const FlaLayerNormArgs* args);
+
 /* Forward pass for callers that cannot obtain device memory themselves.
  * It has no counterpart in the reference (whose wrappers allocate through torch).
  *
