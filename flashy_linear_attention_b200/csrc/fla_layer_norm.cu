@@ -34,13 +34,13 @@ struct LayerNormParams {
   float* parts;           // backward: [CTA][2][heads][d], or null
   long long rows;         // of a head
   int heads, n1, n2, d;   // row j is (j / n2 / n1, j / n2 % n1, j % n2)
-  int lanes;              // that hold a piece (rows of a CTA each)
+  int lanes;              // threads that share a row, where they are whole warps
   float eps;
 };
 
-__device__ __forceinline__ long long row_offset(const NormRows& t, const LayerNormParams& p, long long j, int head) {
-  if (p.n1 == 1 && p.rows == p.n2) return head * t.sh + j * t.s2;
-  const unsigned row = static_cast<unsigned>(j), outer = row / static_cast<unsigned>(p.n2);  // (rows fit 31 bits)
+__device__ __forceinline__ long long row_offset(const NormRows& t, const LayerNormParams& p, unsigned row, int head) {
+  if (p.n1 == 1 && p.rows == p.n2) return head * t.sh + row * t.s2;
+  const unsigned outer = row / static_cast<unsigned>(p.n2);  // (rows fit 31 bits)
   const unsigned i2 = row - outer * p.n2, i0 = outer / static_cast<unsigned>(p.n1), i1 = outer - i0 * p.n1;
   return head * t.sh + i0 * t.s0 + i1 * t.s1 + i2 * t.s2;
 }
@@ -51,325 +51,483 @@ struct Piece {
   static constexpr int kElements = WIDE ? 16 / sizeof(T) : 1;
   using Raw = std::conditional_t<WIDE, uint4, typename PairOf<T>::Element>;
 };
-template <typename T>
-__device__ __forceinline__ void widen(float (&v)[16 / sizeof(T)], const uint4& raw) {
-  if constexpr (sizeof(T) == 4) {
-    v[0] = __uint_as_float(raw.x);
-    v[1] = __uint_as_float(raw.y);
-    v[2] = __uint_as_float(raw.z);
-    v[3] = __uint_as_float(raw.w);
-  } else {
-    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack_pair<T>(words[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
+
+// Loads where `ok`, and leaves the register as it is elsewhere. As one predicated instruction: as a branch or a selection
+// the compiler waited for the loads of later rows before it went on.
+__device__ __forceinline__ void load_if(uint4& r, const char* p, bool ok) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t@p ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+               : "l"(p), "r"(static_cast<int>(ok)));
 }
-template <typename T>
-__device__ __forceinline__ void widen(float (&v)[1], const typename PairOf<T>::Element& raw) {
-  if constexpr (sizeof(T) == 4) v[0] = raw;
-  else v[0] = unpack_pair<T>(static_cast<uint32_t>(raw)).x;
+__device__ __forceinline__ void load_if(float& r, const char* p, bool ok) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p ld.global.nc.f32 %0, [%1];\n\t}"
+               : "+f"(r)
+               : "l"(p), "r"(static_cast<int>(ok)));
 }
-template <typename T>
-__device__ __forceinline__ void narrow(uint4& raw, const float (&v)[16 / sizeof(T)]) {
-  if constexpr (sizeof(T) == 4) {
-    raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  } else {
-    raw = make_uint4(pack_pair<T>(make_float2(v[0], v[1])), pack_pair<T>(make_float2(v[2], v[3])),
-                     pack_pair<T>(make_float2(v[4], v[5])), pack_pair<T>(make_float2(v[6], v[7])));
-  }
-}
-template <typename T>
-__device__ __forceinline__ void narrow(float& raw, const float (&v)[1]) { raw = v[0]; }
-template <typename T>
-__device__ __forceinline__ void narrow(uint16_t& raw, const float (&v)[1]) {
-  raw = static_cast<uint16_t>(pack_pair<T>(make_float2(v[0], 0.f)) & 0xffffu);
+__device__ __forceinline__ void load_if(uint16_t& r, const char* p, bool ok) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p ld.global.nc.b16 %0, [%1];\n\t}"
+               : "+h"(r)
+               : "l"(p), "r"(static_cast<int>(ok)));
 }
 
+// What a thread holds of a row: K pieces, in memory `lanes` pieces apart. In arithmetic the elements go in pairs.
 template <typename T, bool WIDE, int K>
 struct RowRegs {
-  using P = Piece<T, WIDE>;
-  static constexpr int V = P::kElements;
-  typename P::Raw raw[K];
+  using Raw = typename Piece<T, WIDE>::Raw;
+  static constexpr int V = Piece<T, WIDE>::kElements, kPairs = K * V / 2;
+  Raw raw[K];
 
   // Pieces past the row are zero.
   __device__ __forceinline__ void load(const char* row, int lane, int lanes, int d, bool in) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * lanes + lane) * V;
-      raw[k] = typename P::Raw{};
-      if (in && c < d) raw[k] = __ldg(reinterpret_cast<const typename P::Raw*>(row + c * static_cast<int>(sizeof(T))));
+      raw[k] = Raw{};
+      load_if(raw[k], row + c * static_cast<int>(sizeof(T)), in && c < d);
     }
   }
   __device__ __forceinline__ void store(char* row, int lane, int lanes, int d, bool in) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * lanes + lane) * V;
-      if (in && c < d) *reinterpret_cast<typename P::Raw*>(row + c * static_cast<int>(sizeof(T))) = raw[k];
+      if (in && c < d) *reinterpret_cast<Raw*>(row + c * static_cast<int>(sizeof(T))) = raw[k];
+    }
+  }
+  __device__ __forceinline__ void widen(float2 (&v)[kPairs]) const {
+    if constexpr (!WIDE) {
+#pragma unroll
+      for (int k = 0; k < K; k += 2) v[k / 2] = unpack_pair<T>(join_pair(raw[k], raw[k + 1]));
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        v[2 * k] = make_float2(__uint_as_float(raw[k].x), __uint_as_float(raw[k].y));
+        v[2 * k + 1] = make_float2(__uint_as_float(raw[k].z), __uint_as_float(raw[k].w));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        v[4 * k] = unpack_pair<T>(raw[k].x);
+        v[4 * k + 1] = unpack_pair<T>(raw[k].y);
+        v[4 * k + 2] = unpack_pair<T>(raw[k].z);
+        v[4 * k + 3] = unpack_pair<T>(raw[k].w);
+      }
+    }
+  }
+  // Rounded to nearest, once.
+  __device__ __forceinline__ void narrow(const float2 (&v)[kPairs]) {
+    if constexpr (!WIDE) {
+#pragma unroll
+      for (int k = 0; k < K; k += 2) {
+        const auto r = pack_pair<T>(v[k / 2]);
+        raw[k] = reinterpret_cast<const Raw*>(&r)[0];
+        raw[k + 1] = reinterpret_cast<const Raw*>(&r)[1];
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        raw[k] = make_uint4(__float_as_uint(v[2 * k].x), __float_as_uint(v[2 * k].y), __float_as_uint(v[2 * k + 1].x),
+                            __float_as_uint(v[2 * k + 1].y));
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        raw[k] = make_uint4(pack_pair<T>(v[4 * k]), pack_pair<T>(v[4 * k + 1]), pack_pair<T>(v[4 * k + 2]), pack_pair<T>(v[4 * k + 3]));
     }
   }
 };
 
-// A piece of the weights, of the rows' type or fp32.
-template <typename T, int V>
-__device__ __forceinline__ void load_weights(float (&v)[V], const void* w, int wide, long long at, bool in) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = 0.f;
-  if (!in) return;
-  if (wide || sizeof(T) == 4) {
-    const float* f = static_cast<const float*>(w) + at;
-    if constexpr (V == 1) {
-      v[0] = __ldg(f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(f + i));
-        v[i] = q.x;
-        v[i + 1] = q.y;
-        v[i + 2] = q.z;
-        v[i + 3] = q.w;
-      }
-    }
-  } else if constexpr (sizeof(T) == 2) {
-    if constexpr (V == 1) widen<T>(v, __ldg(static_cast<const uint16_t*>(w) + at));
-    else widen<T>(v, __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + at)));
-  }
+// The threads that share a row: LANES of a warp, or (LANES = 0) whole warps, which meet at a barrier of their own.
+struct RowTeam {
+  int lanes, lane, group, groups;
+};
+template <int LANES>
+__device__ __forceinline__ RowTeam row_team(const LayerNormParams& p) {
+  RowTeam t;
+  t.lanes = LANES ? LANES : p.lanes;
+  t.lane = threadIdx.x % t.lanes;
+  t.group = threadIdx.x / t.lanes;
+  t.groups = blockDim.x / t.lanes;
+  return t;
 }
 
-// Sums of N values over the lanes of a row, the same in all of them. LANES = 0: the row has the whole CTA (of up to 32
-// warps); `parts` alternates between two buffers, so that one barrier a sum is enough.
+// Rows that are on their way: every thread copies its pieces of the next kDepth rows of N tensors into slots of its own in
+// shared memory, asynchronously, and reads them back when it gets to the row; no other thread sees them, so there is no
+// barrier. Loads into registers two and four rows ahead did not do: waiting for one of them waits for all behind it
+// (forward, 32768 rows of 4096: 195 us that way). Rows of single elements and the widest ones are loaded directly.
+template <typename T, bool WIDE, int K, int N>
+struct RowsAhead {
+  using Regs = RowRegs<T, WIDE, K>;
+  static constexpr int kElements = K * Regs::V, kBytes = 16 * K;
+  static constexpr bool kStaged = WIDE && kElements <= 32;
+  static constexpr int kDepth = !kStaged ? 1 : kElements <= 8 ? 4 : kElements * sizeof(T) <= 64 ? 2 : 1;
+  uint32_t slot;  // of this thread, in the stage that comes next
+  uint32_t first, last, stage;
+
+  __device__ __forceinline__ explicit RowsAhead(void* shared) {
+    first = slot = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) + threadIdx.x * 16;
+    stage = blockDim.x * kBytes * N;
+    last = first + (kDepth - 1) * stage;
+  }
+  // Starts the copies of a row of tensor n into the stage that comes next. `after`: behind what this value comes from.
+  __device__ __forceinline__ void start(int n, const char* row, const RowTeam& t, int d, bool in, float after) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * t.lanes + t.lane) * Regs::V;
+      const bool ok = in && c < d;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + (n * K + k) * blockDim.x * 16),
+                   "l"(ok ? row + c * static_cast<int>(sizeof(T)) : row), "r"(ok ? 16 : 0), "f"(after)
+                   : "memory");
+    }
+  }
+  __device__ __forceinline__ void next() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot = slot == last ? first : slot + stage;
+  }
+  __device__ __forceinline__ void arrived() const { asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory"); }
+  __device__ __forceinline__ void take(int n, Regs& r) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if constexpr (WIDE)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.raw[k].x), "=r"(r.raw[k].y), "=r"(r.raw[k].z), "=r"(r.raw[k].w)
+                     : "r"(slot + (n * K + k) * blockDim.x * 16)
+                     : "memory");
+  }
+};
+
+// The weights (or biases) of a lane's columns, of the rows' type or fp32; `none` where there are none. In registers for
+// all rows where they are few, else read, from L1, for each row.
+template <typename T, bool WIDE, int K>
+struct LaneWeights {
+  using Regs = RowRegs<T, WIDE, K>;
+  static constexpr int V = Regs::V, kPairs = Regs::kPairs;
+  static constexpr bool kKept = K * V <= 16;
+  float2 v[kKept ? kPairs : 1];
+  const char* p;
+  int wide;
+  float none;
+
+  __device__ __forceinline__ LaneWeights(const void* weights, int w_wide, float if_none, int head, int lane, int lanes, int d) {
+    wide = w_wide || sizeof(T) == 4;
+    p = static_cast<const char*>(weights);
+    if (p != nullptr) p += static_cast<long long>(head) * d * (wide ? 4 : 2);
+    none = if_none;
+    if constexpr (kKept) fetch(v, lane, lanes, d);
+  }
+  __device__ __forceinline__ void fetch(float2 (&w)[kPairs], int lane, int lanes, int d) const {
+    if (p == nullptr) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) w[i] = make_float2(none, none);
+    } else if (!wide) {
+      Regs r;
+      r.load(p, lane, lanes, d, true);
+      r.widen(w);
+    } else if constexpr (!WIDE) {
+      RowRegs<float, false, K> r;
+      r.load(p, lane, lanes, d, true);
+      r.widen(w);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * lanes + lane) * V;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+          const float4 q = c < d ? __ldg(reinterpret_cast<const float4*>(p + (c + i) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          w[(k * V + i) / 2] = make_float2(q.x, q.y);
+          w[(k * V + i) / 2 + 1] = make_float2(q.z, q.w);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float2 (&w)[kPairs], int lane, int lanes, int d) const {
+    if constexpr (kKept) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) w[i] = v[i];
+    } else {
+      fetch(w, lane, lanes, d);
+    }
+  }
+};
+
+// Sums of N values over a row, the same in all of its threads. `parts`, of 32 words a value and turn for all groups
+// together, alternates between two turns, so that one barrier a sum is enough.
 template <int LANES, int N>
-__device__ __forceinline__ void sum_over_row(float (&v)[N], float (*parts)[2][32], int& turn) {
+__device__ __forceinline__ void sum_over_row(float (&v)[N], float (*parts)[N][32], int& turn, const RowTeam& t) {
   constexpr int kSpan = LANES ? LANES : 32;
 #pragma unroll
   for (int o = kSpan / 2; o > 0; o /= 2)
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   if constexpr (LANES == 0) {
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-    if (lane == 0)
+    const int warp = threadIdx.x / 32, warps = t.lanes / 32;
+    if (threadIdx.x % 32 == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) parts[turn][i][warp] = v[i];
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(t.group + 1), "r"(t.lanes) : "memory");
+    const int w = threadIdx.x % 16;  // (a row has 16 warps at most)
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lane < warps ? parts[turn][i][lane] : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = w < warps ? parts[turn][i][t.group * warps + w] : 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2)
+    for (int o = 8; o > 0; o /= 2)
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     turn ^= 1;
   }
 }
 
-constexpr int kNormGroupThreads = 256;  // of a CTA whose rows have 32 lanes or fewer
+// 1 / sqrt(v): the fast instruction, off by 2^-22, and a Newton step on it, which brings that to a rounding or two.
+__device__ __forceinline__ float reciprocal_root(float v) {
+  const float r = rsqrtf(v);
+  return v > 0.f && v < 3e38f ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Threads a CTA at most, for K pieces a thread (rows of a CTA each).
-constexpr int norm_cta_threads(int k) { return k <= 2 ? 512 : 1024; }
+// Registers decide how many threads an SM holds: up to 8 elements of a row a thread leave room for 1024 (backward, with
+// two rows in fp32 at a time and the sums of the weights' gradients, 768), more for 512.
+__host__ __device__ constexpr int norm_threads_sm(bool backward, int values) { return values > 8 ? 512 : backward ? 768 : 1024; }
+__host__ __device__ constexpr int norm_threads_cta(bool backward, int values) { return values <= 8 && backward ? 256 : 512; }
 
+// The next rows are on their way while these are worked on.
 template <typename T, bool WIDE, int LANES, int K>
-__global__ void __launch_bounds__(LANES ? kNormGroupThreads : norm_cta_threads(K), 1) fla_layer_norm_fwd_kernel(const LayerNormParams p) {
+__global__ void __launch_bounds__(norm_threads_cta(false, K * Piece<T, WIDE>::kElements), norm_threads_sm(false, K * Piece<T, WIDE>::kElements) / norm_threads_cta(false, K * Piece<T, WIDE>::kElements))
+fla_layer_norm_fwd_kernel(const LayerNormParams p) {
   using Regs = RowRegs<T, WIDE, K>;
-  constexpr int V = Regs::V;
-  __shared__ float parts[2][2][32];
+  constexpr int V = Regs::V, P = Regs::kPairs;
+  __shared__ float parts[2][1][32];
   int turn = 0;
-  const int lanes = LANES ? LANES : static_cast<int>(blockDim.x), lane = threadIdx.x % lanes;
-  const int groups = blockDim.x / lanes, head = blockIdx.y;
+  const RowTeam t = row_team<LANES>(p);
+  const int head = blockIdx.y;
+  const unsigned rows = static_cast<unsigned>(p.rows), stride = gridDim.x * t.groups;
   const float over_d = 1.f / p.d;
-  // (every lane of a warp, and of a CTA that shares rows, takes the same turns)
-  for (long long base = static_cast<long long>(blockIdx.x) * groups; base < p.rows; base += static_cast<long long>(gridDim.x) * groups) {
-    const long long j = base + threadIdx.x / lanes;
-    const bool in = j < p.rows;
-    Regs x;
-    x.load(p.x.ptr + (in ? row_offset(p.x, p, j, head) : 0), lane, lanes, p.d, in);
-    float v[K][V], sum[1] = {0.f};
+  const bool whole = t.lanes * K * V == p.d;  // no thread has pieces past the row
+  const LaneWeights<T, WIDE, K> weight(p.w, p.w_wide, 1.f, head, t.lane, t.lanes, p.d), bias(p.b, p.w_wide, 0.f, head, t.lane, t.lanes, p.d);
+  extern __shared__ uint4 slots[];
+  using Ahead = RowsAhead<T, WIDE, K, 2>;
+  Ahead ahead(slots);
+  Regs x, z;
+  unsigned next = blockIdx.x * t.groups + t.group;
+  auto fetch = [&](float after) {  // the row after those that are on their way
+    const bool in = next < rows;
+    const char* xr = p.x.ptr + (in ? row_offset(p.x, p, next, head) : 0);
+    const char* zr = p.z.ptr + (in && p.z.ptr != nullptr ? row_offset(p.z, p, next, head) : 0);
+    if constexpr (Ahead::kStaged) {
+      ahead.start(0, xr, t, p.d, in, after);
+      if (p.z.ptr != nullptr) ahead.start(1, zr, t, p.d, in, after);
+      ahead.next();
+    } else {
+      x.load(xr, t.lane, t.lanes, p.d, in);
+      if (p.z.ptr != nullptr) z.load(zr, t.lane, t.lanes, p.d, in);
+    }
+    next += stride;
+  };
+#pragma unroll
+  for (int s = 0; s < Ahead::kDepth; ++s) fetch(0.f);
+  unsigned j = blockIdx.x * t.groups + t.group;
+  // (every lane of a warp takes the same turns: its first row decides)
+  for (unsigned base = blockIdx.x * t.groups; base < rows; base += stride, j += stride) {
+    const bool in = j < rows;
+    if constexpr (Ahead::kStaged) {
+      ahead.arrived();
+      ahead.take(0, x);
+      if (p.z.ptr != nullptr) ahead.take(1, z);
+    }
+    float2 v[P];
     if (p.z.ptr != nullptr) {
-      Regs z;
-      z.load(p.z.ptr + (in ? row_offset(p.z, p, j, head) : 0), lane, lanes, p.d, in);
+      float2 more[P];
+      x.widen(v);
+      z.widen(more);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float a[V], b[V];
-        widen<T>(a, x.raw[k]);
-        widen<T>(b, z.raw[k]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) a[i] += b[i];
-        narrow<T>(x.raw[k], a);  // what is normalised is the sum as it is stored
-      }
-      x.store(p.s.ptr + (in ? row_offset(p.s, p, j, head) : 0), lane, lanes, p.d, in);
+      for (int i = 0; i < P; ++i) v[i] = add2(v[i], more[i]);
+      x.narrow(v);  // what is normalised is the sum as it is stored
+      x.store(p.s.ptr + (in ? row_offset(p.s, p, j, head) : 0), t.lane, t.lanes, p.d, in);
     }
+    x.widen(v);
+    float2 pair = v[0];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      widen<T>(v[k], x.raw[k]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum[0] += v[k][i];
-    }
-    sum_over_row<LANES>(sum, parts, turn);
+    for (int i = 1; i < P; ++i) pair = add2(pair, v[i]);
+    float sum[1] = {pair.x + pair.y};
+    fetch(sum[0]);
+    sum_over_row<LANES>(sum, parts, turn, t);
     const float mean = sum[0] * over_d;
-    float square[1] = {0.f};
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int i = 0; i < P; ++i) v[i] = add2(v[i], both(-mean));
+    if (!whole) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[k][i] -= mean;
-        if ((k * lanes + lane) * V < p.d) square[0] = fmaf(v[k][i], v[k][i], square[0]);
+      for (int i = 0; i < P; ++i) {
+        if ((2 * i / V * t.lanes + t.lane) * V >= p.d) v[i].x = 0.f;
+        if (((2 * i + 1) / V * t.lanes + t.lane) * V >= p.d) v[i].y = 0.f;
       }
-    sum_over_row<LANES>(square, parts, turn);
-    const float r = 1.f / sqrtf(square[0] * over_d + p.eps);
-    if (p.stats != nullptr && lane == 0 && in)
-      *reinterpret_cast<float2*>(p.stats + 2 * (head * p.rows + j)) = make_float2(mean, r);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * lanes + lane) * V;
-      const long long at = static_cast<long long>(head) * p.d + c;
-      float w[V], b[V];
-      if (p.w != nullptr) load_weights<T>(w, p.w, p.w_wide, at, c < p.d);
-      if (p.b != nullptr) load_weights<T>(b, p.b, p.w_wide, at, c < p.d);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float y = v[k][i] * r;
-        if (p.w != nullptr) y *= w[i];
-        if (p.b != nullptr) y += b[i];
-        v[k][i] = y;
-      }
-      narrow<T>(x.raw[k], v[k]);
     }
-    x.store(p.y.ptr + (in ? row_offset(p.y, p, j, head) : 0), lane, lanes, p.d, in);
+    pair = mul2(v[0], v[0]);
+#pragma unroll
+    for (int i = 1; i < P; ++i) pair = fma2(v[i], v[i], pair);
+    sum[0] = pair.x + pair.y;
+    sum_over_row<LANES>(sum, parts, turn, t);
+    const float r = reciprocal_root(fmaf(sum[0], over_d, p.eps));
+    if (p.stats != nullptr && t.lane == 0 && in)
+      *reinterpret_cast<float2*>(p.stats + 2 * (head * p.rows + j)) = make_float2(mean, r);
+    Regs y;
+    float2 w[P], b[P];
+    weight.get(w, t.lane, t.lanes, p.d);
+    bias.get(b, t.lane, t.lanes, p.d);
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = fma2(mul2(v[i], both(r)), w[i], b[i]);
+    y.narrow(v);
+    y.store(p.y.ptr + (in ? row_offset(p.y, p, j, head) : 0), t.lane, t.lanes, p.d, in);
   }
 }
 
 template <typename T, bool WIDE, int LANES, int K>
-__global__ void __launch_bounds__(LANES ? kNormGroupThreads : norm_cta_threads(K), 1) fla_layer_norm_bwd_kernel(const LayerNormParams p) {
+__global__ void __launch_bounds__(norm_threads_cta(true, K * Piece<T, WIDE>::kElements), norm_threads_sm(true, K * Piece<T, WIDE>::kElements) / norm_threads_cta(true, K * Piece<T, WIDE>::kElements))
+fla_layer_norm_bwd_kernel(const LayerNormParams p) {
   using Regs = RowRegs<T, WIDE, K>;
-  constexpr int V = Regs::V;
+  constexpr int V = Regs::V, P = Regs::kPairs;
   __shared__ float parts[2][2][32];
-  extern __shared__ float joined[];  // [2][d], where a CTA has several rows at a time
   int turn = 0;
-  const int lanes = LANES ? LANES : static_cast<int>(blockDim.x), lane = threadIdx.x % lanes;
-  const int groups = blockDim.x / lanes, head = blockIdx.y;
+  const RowTeam t = row_team<LANES>(p);
+  const int head = blockIdx.y;
+  const unsigned rows = static_cast<unsigned>(p.rows), stride = gridDim.x * t.groups;
   const float over_d = 1.f / p.d;
-  float dw[K][V], db[K][V];
+  const LaneWeights<T, WIDE, K> weight(p.w, p.w_wide, 1.f, head, t.lane, t.lanes, p.d);
+  float2 dw[P], db[P];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
-  for (long long base = static_cast<long long>(blockIdx.x) * groups; base < p.rows; base += static_cast<long long>(gridDim.x) * groups) {
-    const long long j = base + threadIdx.x / lanes;
-    const bool in = j < p.rows;
-    Regs x, dy;
-    x.load(p.x.ptr + (in ? row_offset(p.x, p, j, head) : 0), lane, lanes, p.d, in);
-    dy.load(p.dy.ptr + (in ? row_offset(p.dy, p, j, head) : 0), lane, lanes, p.d, in);
-    const float2 stats = in ? __ldg(reinterpret_cast<const float2*>(p.stats + 2 * (head * p.rows + j))) : make_float2(0.f, 0.f);
-    float sums[2] = {0.f, 0.f};  // of u and of u n
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * lanes + lane) * V;
-      float n[V], g[V], w[V];
-      widen<T>(n, x.raw[k]);
-      widen<T>(g, dy.raw[k]);
-      if (p.w != nullptr) load_weights<T>(w, p.w, p.w_wide, static_cast<long long>(head) * p.d + c, c < p.d);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        n[i] = (n[i] - stats.x) * stats.y;
-        if (in) dw[k][i] = fmaf(g[i], n[i], dw[k][i]);
-        db[k][i] += g[i];
-        const float u = p.w != nullptr ? g[i] * w[i] : g[i];
-        sums[0] += u;
-        sums[1] = fmaf(u, n[i], sums[1]);
-      }
+  for (int i = 0; i < P; ++i) dw[i] = db[i] = both(0.f);
+  extern __shared__ uint4 slots[];  // rows on their way; then [2][d] sums, where a CTA has several rows at a time
+  using Ahead = RowsAhead<T, WIDE, K, 3>;
+  Ahead ahead(slots);
+  Regs x, dy, ds;
+  float2 stats;
+  const unsigned start = blockIdx.x * t.groups + t.group;
+  unsigned next = start, stats_next = start;
+  auto fetch = [&](float after) {  // the row after those that are on their way
+    const bool in = next < rows;
+    const char* xr = p.x.ptr + (in ? row_offset(p.x, p, next, head) : 0);
+    const char* gr = p.dy.ptr + (in ? row_offset(p.dy, p, next, head) : 0);
+    if constexpr (Ahead::kStaged) {
+      ahead.start(0, xr, t, p.d, in, after);
+      ahead.start(1, gr, t, p.d, in, after);
+      if (p.ds.ptr != nullptr) ahead.start(2, p.ds.ptr + (in ? row_offset(p.ds, p, next, head) : 0), t, p.d, in, after);
+      ahead.next();
+    } else {
+      x.load(xr, t.lane, t.lanes, p.d, in);
+      dy.load(gr, t.lane, t.lanes, p.d, in);
     }
+    next += stride;
+  };
+  auto fetch_stats = [&] {
+    stats = stats_next < rows ? __ldg(reinterpret_cast<const float2*>(p.stats + 2 * (head * p.rows + stats_next))) : both(0.f);
+    stats_next += stride;
+  };
+  fetch_stats();
+#pragma unroll
+  for (int s = 0; s < Ahead::kDepth; ++s) fetch(0.f);
+  unsigned j = start;
+  for (unsigned base = blockIdx.x * t.groups; base < rows; base += stride, j += stride) {
+    const bool in = j < rows;
+    if constexpr (Ahead::kStaged) {
+      ahead.arrived();
+      ahead.take(0, x);
+      ahead.take(1, dy);
+      if (p.ds.ptr != nullptr) ahead.take(2, ds);
+    } else {
+      if (p.ds.ptr != nullptr) ds.load(p.ds.ptr + (in ? row_offset(p.ds, p, j, head) : 0), t.lane, t.lanes, p.d, in);
+    }
+    const float r = stats.y;
+    const float2 shift = both(-stats.x);
+    // (where there is no row, dy and r are zero, and past the end of a row dy: nothing is added)
+    float2 n[P], u[P], w[P];
+    x.widen(n);
+    dy.widen(u);
+    fetch_stats();
+    weight.get(w, t.lane, t.lanes, p.d);
+    float2 s0 = both(0.f), s1 = s0;  // of u and of u n
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      n[i] = mul2(add2(n[i], shift), both(r));
+      dw[i] = fma2(u[i], n[i], dw[i]);
+      db[i] = add2(db[i], u[i]);
+      u[i] = mul2(u[i], w[i]);
+      s0 = add2(s0, u[i]);
+      s1 = fma2(u[i], n[i], s1);
+    }
+    float sums[2] = {s0.x + s0.y, s1.x + s1.y};
+    fetch(sums[1]);
     if (p.dx.ptr == nullptr) continue;
-    sum_over_row<LANES>(sums, parts, turn);
-    const float mean_u = sums[0] * over_d, mean_un = sums[1] * over_d;
-    Regs ds;
-    if (p.ds.ptr != nullptr) ds.load(p.ds.ptr + (in ? row_offset(p.ds, p, j, head) : 0), lane, lanes, p.d, in);
+    sum_over_row<LANES>(sums, parts, turn, t);
+    const float2 mean_u = both(-sums[0] * over_d), mean_un = both(-sums[1] * over_d);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * lanes + lane) * V;
-      float n[V], g[V], w[V], more[V];
-      widen<T>(n, x.raw[k]);
-      widen<T>(g, dy.raw[k]);
-      if (p.w != nullptr) load_weights<T>(w, p.w, p.w_wide, static_cast<long long>(head) * p.d + c, c < p.d);
-      if (p.ds.ptr != nullptr) widen<T>(more, ds.raw[k]);
+    for (int i = 0; i < P; ++i) u[i] = mul2(fma2(n[i], mean_un, add2(u[i], mean_u)), both(r));
+    if (p.ds.ptr != nullptr) {
+      ds.widen(w);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        n[i] = (n[i] - stats.x) * stats.y;
-        const float u = p.w != nullptr ? g[i] * w[i] : g[i];
-        g[i] = stats.y * (u - mean_u - n[i] * mean_un);
-        if (p.ds.ptr != nullptr) g[i] += more[i];
-      }
-      narrow<T>(x.raw[k], g);
+      for (int i = 0; i < P; ++i) u[i] = add2(u[i], w[i]);
     }
-    x.store(p.dx.ptr + (in ? row_offset(p.dx, p, j, head) : 0), lane, lanes, p.d, in);
+    Regs dx;
+    dx.narrow(u);
+    dx.store(p.dx.ptr + (in ? row_offset(p.dx, p, j, head) : 0), t.lane, t.lanes, p.d, in);
   }
   if (p.parts == nullptr) return;
   float* out = p.parts + (static_cast<long long>(blockIdx.x) * 2 * p.heads + head) * p.d;  // dw; db lies heads * d behind
   const long long db_at = static_cast<long long>(p.heads) * p.d;
-  if constexpr (LANES == 0) {
+  // The groups of a warp join by shuffles, then warps or groups of warps one after the other.
+  constexpr int kSpan = LANES ? 32 : 0;
+  float* const joined = reinterpret_cast<float*>(slots);
+  if constexpr (Ahead::kStaged) asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // (the slots are free)
+  if constexpr (LANES != 0)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int i = 0; i < P; ++i)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = (k * lanes + lane) * V + i;
+      for (int o = LANES; o < 32; o *= 2) {
+        dw[i] = add2(dw[i], make_float2(__shfl_xor_sync(0xffffffffu, dw[i].x, o), __shfl_xor_sync(0xffffffffu, dw[i].y, o)));
+        db[i] = add2(db[i], make_float2(__shfl_xor_sync(0xffffffffu, db[i].x, o), __shfl_xor_sync(0xffffffffu, db[i].y, o)));
+      }
+  const int team = kSpan ? threadIdx.x / 32 : t.group, teams = kSpan ? static_cast<int>(blockDim.x) / 32 : t.groups;
+  for (int turn_of = 0; turn_of < teams; ++turn_of) {
+    if (team == turn_of && (LANES == 0 || threadIdx.x % 32 < LANES)) {
+      float* const w_to = teams > 1 ? joined : out;
+      float* const b_to = teams > 1 ? joined + p.d : out + db_at;
+#pragma unroll
+      for (int e = 0; e < 2 * P; ++e) {
+        const int c = (e / V * t.lanes + t.lane) * V + e % V;
+        const float ew = e % 2 ? dw[e / 2].y : dw[e / 2].x, eb = e % 2 ? db[e / 2].y : db[e / 2].x;
         if (c < p.d) {
-          out[c] = dw[k][i];
-          out[db_at + c] = db[k][i];
+          w_to[c] = turn_of ? w_to[c] + ew : ew;
+          b_to[c] = turn_of ? b_to[c] + eb : eb;
         }
       }
-  } else {
-    const int warp = threadIdx.x / 32;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-#pragma unroll
-        for (int o = LANES; o < 32; o *= 2) {
-          dw[k][i] += __shfl_xor_sync(0xffffffffu, dw[k][i], o);
-          db[k][i] += __shfl_xor_sync(0xffffffffu, db[k][i], o);
-        }
-    for (int turn_of = 0; turn_of < static_cast<int>(blockDim.x) / 32; ++turn_of) {
-      if (warp == turn_of && threadIdx.x % 32 < LANES) {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int c = (k * lanes + lane) * V + i;
-            if (c < p.d) {
-              joined[c] = turn_of ? joined[c] + dw[k][i] : dw[k][i];
-              joined[p.d + c] = turn_of ? joined[p.d + c] + db[k][i] : db[k][i];
-            }
-          }
-      }
-      __syncthreads();
     }
+    __syncthreads();
+  }
+  if (teams > 1)
     for (int c = threadIdx.x; c < p.d; c += blockDim.x) {
       out[c] = joined[c];
       out[db_at + c] = joined[p.d + c];
     }
-  }
 }
 
-// dw and db from the CTAs' sums: 32 columns a block, eight shares of the CTAs side by side, joined in order.
+// dw and db from the CTAs' sums: 32 columns a block, 32 shares of the CTAs side by side, joined in order.
 template <typename W>
-__global__ void __launch_bounds__(256) fla_layer_norm_weights_kernel(const float* parts, int ctas, int columns, W* dw, W* db) {
-  __shared__ float shares[8][32];
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, share = threadIdx.x / 32;
+__global__ void __launch_bounds__(1024) fla_layer_norm_weights_kernel(const float* parts, int ctas, int columns, W* dw, W* db) {
+  __shared__ float shares[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x, share = threadIdx.y;
   W* out = blockIdx.y ? db : dw;
   if (out == nullptr) return;
   float sum = 0.f;
   if (c < columns) {
     const float* at = parts + static_cast<long long>(blockIdx.y) * columns + c;
-#pragma unroll 8
-    for (int i = share; i < ctas; i += 8) sum += __ldg(at + static_cast<long long>(i) * 2 * columns);
+#pragma unroll 4
+    for (int i = share; i < ctas; i += 32) sum += __ldg(at + static_cast<long long>(i) * 2 * columns);
   }
-  shares[share][threadIdx.x % 32] = sum;
+  shares[share][threadIdx.x] = sum;
   __syncthreads();
-  if (share == 0 && c < columns) {
+  // a warp a column now
+  sum = shares[threadIdx.x][share];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += shares[i][threadIdx.x];
-    if constexpr (sizeof(W) == 4) out[c] = sum;
-    else out[c] = static_cast<W>(sum);
+  for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int mine = blockIdx.x * 32 + share;
+  if (threadIdx.x == 0 && mine < columns) {
+    if constexpr (sizeof(W) == 4) out[mine] = sum;
+    else out[mine] = static_cast<W>(sum);
   }
 }
 
@@ -387,7 +545,7 @@ int norm_element(int dtype) { return dtype == FLA_DTYPE_F32 ? 4 : 2; }
 struct NormPlan {
   LayerNormParams p;
   bool wide;
-  int lanes, k;      // lanes: 0 where a row has a CTA
+  int lanes, k;       // lanes: 0 where a row has whole warps, p.lanes threads
   int threads, ctas;  // ctas: of a head
 };
 
@@ -457,26 +615,22 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
                 return aligned(t.ptr, 16) && (p.heads == 1 || t.sh % 16 == 0) && (n0 == 1 || t.s0 % 16 == 0) &&
                        (p.n1 == 1 || t.s1 % 16 == 0) && (p.n2 == 1 || t.s2 % 16 == 0);
               });
+  // A thread holds up to 8 elements of a row, backward of rows above 1024 columns 16; 16, 32 or 64 of the widest.
   const int pieces = plan.wide ? p.d / per : p.d;
-  if (plan.wide) {
-    if (pieces <= 128) {
-      plan.lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
-      plan.k = pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4;
-    } else {
-      plan.k = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : pieces <= 4096 ? 4 : 8;
-    }
-  } else if (pieces <= 512) {
-    plan.lanes = 32;
-    plan.k = pieces <= 32 ? 1 : pieces <= 128 ? 4 : 16;
-  } else {
-    plan.k = pieces <= 8192 ? 8 : 32;
-  }
-  plan.threads = plan.lanes ? fla::kNormGroupThreads : (pieces + plan.k * 32 - 1) / (plan.k * 32) * 32;
-  const long long groups = plan.lanes ? plan.threads / plan.lanes : 1;
-  // As many CTAs as are resident together; a CTA of the backward leaves a row of sums behind, so it has 8 rows or more.
-  const long long most = std::max<long long>(1, static_cast<long long>(sm_count) * (2048 / plan.threads) / (backward ? 2 : 1) / p.heads);
+  const int held = plan.wide ? per : 1;
+  const int values = p.d <= (backward ? 1024 : 4096) ? 8 : p.d <= 8192 ? 16 : p.d <= 16384 ? 32 : 64;
+  plan.k = values / held;
+  if (plan.wide && pieces <= 32) plan.k = 1;
+  if (!plan.wide && pieces <= 128) plan.k = pieces <= 64 ? 2 : 4;
+  plan.lanes = plan.wide && pieces <= 8 ? 8 : plan.wide && pieces <= 16 ? 16 : pieces <= 32 * plan.k ? 32 : 0;
+  p.lanes = plan.lanes ? plan.lanes : (pieces + plan.k * 32 - 1) / (plan.k * 32) * 32;
+  const long long groups = std::max(1, 256 / p.lanes);
+  plan.threads = static_cast<int>(groups) * p.lanes;
+  // As many CTAs as are resident together; a CTA of the backward leaves a row of sums behind, so it has two turns or more.
+  const int resident = std::max(1, fla::norm_threads_sm(backward, plan.k * held) / plan.threads);
+  const long long most = std::max<long long>(1, static_cast<long long>(sm_count) * resident / p.heads);
   const long long turns = (p.rows + groups - 1) / groups;
-  plan.ctas = static_cast<int>(std::min(most, backward ? (turns + 7) / 8 : turns));
+  plan.ctas = static_cast<int>(std::min(most, backward ? (turns + 1) / 2 : turns));
   return plan;
 }
 
@@ -484,35 +638,41 @@ size_t norm_workspace(const NormPlan& plan) { return static_cast<size_t>(plan.ct
 
 template <typename T, bool WIDE, int LANES, int K>
 int norm_launch(const NormPlan& plan, bool backward, cudaStream_t stream) {
+  using Ahead = fla::RowsAhead<T, WIDE, K, 1>;
   const dim3 grid(plan.ctas, plan.p.heads);
-  if (backward) {
-    const int shared = LANES && plan.p.parts != nullptr ? 2 * plan.p.d * static_cast<int>(sizeof(float)) : 0;
-    fla::fla_layer_norm_bwd_kernel<T, WIDE, LANES, K><<<grid, plan.threads, shared, stream>>>(plan.p);
-    return fla::launched(cudaSuccess, "fla_layer_norm_bwd_kernel");
-  }
-  fla::fla_layer_norm_fwd_kernel<T, WIDE, LANES, K><<<grid, plan.threads, 0, stream>>>(plan.p);
-  return fla::launched(cudaSuccess, "fla_layer_norm_fwd_kernel");
+  const auto kernel = backward ? fla::fla_layer_norm_bwd_kernel<T, WIDE, LANES, K> : fla::fla_layer_norm_fwd_kernel<T, WIDE, LANES, K>;
+  // (the stages are laid out for the most tensors that a row can have)
+  size_t shared = Ahead::kStaged ? static_cast<size_t>(Ahead::kDepth) * Ahead::kBytes * plan.threads * (backward ? 3 : 2) : 0;
+  if (backward && plan.p.parts != nullptr && plan.threads > std::max(32, plan.p.lanes))
+    shared = std::max(shared, 2 * plan.p.d * sizeof(float));
+  if (shared > 40 * 1024 &&  // (48 KB go without, with what the kernels declare)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess)
+    return FLA_ERR_CUDA;
+  kernel<<<grid, plan.threads, shared, stream>>>(plan.p);
+  return fla::launched(cudaSuccess, backward ? "fla_layer_norm_bwd_kernel" : "fla_layer_norm_fwd_kernel");
 }
 
 template <typename T>
 int norm_launch_type(const NormPlan& plan, bool backward, cudaStream_t stream) {
+  constexpr int kPer = 16 / sizeof(T), k8 = 8 / kPer;  // elements of a piece, pieces of 8 elements
   if (plan.wide) {
     if (plan.lanes == 8) return norm_launch<T, true, 8, 1>(plan, backward, stream);
     if (plan.lanes == 16) return norm_launch<T, true, 16, 1>(plan, backward, stream);
     if (plan.lanes == 32 && plan.k == 1) return norm_launch<T, true, 32, 1>(plan, backward, stream);
-    if (plan.lanes == 32 && plan.k == 2) return norm_launch<T, true, 32, 2>(plan, backward, stream);
-    if (plan.lanes == 32) return norm_launch<T, true, 32, 4>(plan, backward, stream);
-    if (plan.k == 1) return norm_launch<T, true, 0, 1>(plan, backward, stream);
-    if (plan.k == 2) return norm_launch<T, true, 0, 2>(plan, backward, stream);
-    if (plan.k == 4) return norm_launch<T, true, 0, 4>(plan, backward, stream);
-    if constexpr (sizeof(T) == 4) return norm_launch<T, true, 0, 8>(plan, backward, stream);
-    return FLA_ERR_UNSUPPORTED;
+    if constexpr (k8 > 1)
+      if (plan.lanes == 32) return norm_launch<T, true, 32, k8>(plan, backward, stream);
+    if (plan.k == k8) return norm_launch<T, true, 0, k8>(plan, backward, stream);
+    if (plan.k == 2 * k8) return norm_launch<T, true, 0, 2 * k8>(plan, backward, stream);
+    if (plan.k == 4 * k8) return norm_launch<T, true, 0, 4 * k8>(plan, backward, stream);
+    return norm_launch<T, true, 0, 8 * k8>(plan, backward, stream);
   }
-  if (plan.lanes && plan.k == 1) return norm_launch<T, false, 32, 1>(plan, backward, stream);
+  if (plan.lanes && plan.k == 2) return norm_launch<T, false, 32, 2>(plan, backward, stream);
   if (plan.lanes && plan.k == 4) return norm_launch<T, false, 32, 4>(plan, backward, stream);
-  if (plan.lanes) return norm_launch<T, false, 32, 16>(plan, backward, stream);
+  if (plan.lanes) return norm_launch<T, false, 32, 8>(plan, backward, stream);
   if (plan.k == 8) return norm_launch<T, false, 0, 8>(plan, backward, stream);
-  return norm_launch<T, false, 0, 32>(plan, backward, stream);
+  if (plan.k == 16) return norm_launch<T, false, 0, 16>(plan, backward, stream);
+  if (plan.k == 32) return norm_launch<T, false, 0, 32>(plan, backward, stream);
+  return norm_launch<T, false, 0, 64>(plan, backward, stream);
 }
 
 int norm_dispatch(const FlaLayerNormArgs* a, const NormPlan& plan, bool backward) {
@@ -579,13 +739,13 @@ int fla_sm100_layer_norm_bwd(const FlaLayerNormArgs* a) {
   const dim3 grid((columns + 31) / 32, 2);
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   if (a->w_dtype == FLA_DTYPE_F32)
-    fla::fla_layer_norm_weights_kernel<<<grid, 256, 0, stream>>>(plan.p.parts, plan.ctas, columns, static_cast<float*>(a->d_weight),
+    fla::fla_layer_norm_weights_kernel<<<grid, dim3(32, 32), 0, stream>>>(plan.p.parts, plan.ctas, columns, static_cast<float*>(a->d_weight),
                                                                 static_cast<float*>(a->d_bias));
   else if (a->w_dtype == FLA_DTYPE_F16)
-    fla::fla_layer_norm_weights_kernel<<<grid, 256, 0, stream>>>(plan.p.parts, plan.ctas, columns, static_cast<__half*>(a->d_weight),
+    fla::fla_layer_norm_weights_kernel<<<grid, dim3(32, 32), 0, stream>>>(plan.p.parts, plan.ctas, columns, static_cast<__half*>(a->d_weight),
                                                                 static_cast<__half*>(a->d_bias));
   else
-    fla::fla_layer_norm_weights_kernel<<<grid, 256, 0, stream>>>(plan.p.parts, plan.ctas, columns,
+    fla::fla_layer_norm_weights_kernel<<<grid, dim3(32, 32), 0, stream>>>(plan.p.parts, plan.ctas, columns,
                                                                 static_cast<__nv_bfloat16*>(a->d_weight),
                                                                 static_cast<__nv_bfloat16*>(a->d_bias));
   return fla::launched(cudaSuccess, "fla_layer_norm_weights_kernel");

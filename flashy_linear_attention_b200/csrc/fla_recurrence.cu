@@ -113,25 +113,6 @@ __device__ __forceinline__ RunMap run_map(float2 sum, float2 b) {
   return m;
 }
 
-// Two channels at once: sm_100 multiplies and adds pairs of floats in one instruction.
-__device__ __forceinline__ uint64_t bits(float2 v) { return *reinterpret_cast<const uint64_t*>(&v); }
-__device__ __forceinline__ float2 floats(uint64_t v) { return *reinterpret_cast<const float2*>(&v); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return floats(d);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return floats(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return floats(d);
-}
-
 // Decays of one token. 16-bit rows: the fast exponential, whose error acts on the tokens of a run only.
 template <typename TX>
 __device__ __forceinline__ float2 decay(float2 g) {
