@@ -7,7 +7,7 @@
 // heads is the usual alternative to the denominator of README.md:27-30.
 //
 // Bound by HBM: a row is read once, into registers, and everything that is summed over it is summed from there (the
-// variance from differences to the mean: no cancellation). A row has a group of 8, 16 or 32 lanes, the smallest whose
+// variance from differences to the mean: no cancellation). A row has a group of 4 to 32 lanes, the smallest whose
 // 16-byte pieces cover it (four to a lane at most), or a CTA where it is longer. Backward, a group adds
 // up its rows' dy n and dy in registers, the groups of a CTA join theirs in shared memory, and a second kernel sums the
 // CTAs'. All orders are fixed.
@@ -38,12 +38,36 @@ struct LayerNormParams {
   float eps;
 };
 
-__device__ __forceinline__ long long row_offset(const NormRows& t, const LayerNormParams& p, unsigned row, int head) {
-  if (p.n1 == 1 && p.rows == p.n2) return head * t.sh + row * t.s2;
-  const unsigned outer = row / static_cast<unsigned>(p.n2);  // (rows fit 31 bits)
-  const unsigned i2 = row - outer * p.n2, i0 = outer / static_cast<unsigned>(p.n1), i1 = outer - i0 * p.n1;
-  return head * t.sh + i0 * t.s0 + i1 * t.s1 + i2 * t.s2;
-}
+// The rows that a group of threads works on, one after the other: their numbers are `step` apart. FLAT: all rows of a head
+// are one stride apart in every tensor, and addresses are advanced, not worked out (64-bit products and a division for
+// each row and tensor were a third of the instructions).
+template <bool FLAT>
+struct Cursor {
+  char* at;         // FLAT: the row's address
+  const NormRows* t;
+  long long step_bytes;
+  long long of_head;
+
+  __device__ __forceinline__ Cursor(const NormRows& rows, int head, unsigned row, unsigned step) {
+    t = &rows;
+    of_head = head * rows.sh;
+    if (FLAT) {
+      at = rows.ptr + of_head + row * rows.s2;
+      step_bytes = step * rows.s2;
+    }
+  }
+  // Row `row`, which has to be the one that the cursor has been advanced to.
+  __device__ __forceinline__ char* get(const LayerNormParams& p, unsigned row, bool in) const {
+    if (FLAT) return at;
+    if (!in) return t->ptr;
+    const unsigned outer = row / static_cast<unsigned>(p.n2), i2 = row - outer * p.n2;
+    const unsigned i0 = outer / static_cast<unsigned>(p.n1), i1 = outer - i0 * p.n1;
+    return t->ptr + (of_head + i0 * t->s0 + i1 * t->s1 + i2 * t->s2);
+  }
+  __device__ __forceinline__ void advance() {
+    if (FLAT) at += step_bytes;
+  }
+};
 
 // A piece of a row: 16 bytes, or one element where rows are not aligned or end inside a piece.
 template <typename T, bool WIDE>
@@ -152,18 +176,19 @@ __device__ __forceinline__ RowTeam row_team(const LayerNormParams& p) {
 // Rows that are on their way: every thread copies its pieces of the next kDepth rows of N tensors into slots of its own in
 // shared memory, asynchronously, and reads them back when it gets to the row; no other thread sees them, so there is no
 // barrier. Loads into registers two and four rows ahead did not do: waiting for one of them waits for all behind it
-// (forward, 32768 rows of 4096: 195 us that way). Rows of single elements and the widest ones are loaded directly.
+// (forward, 32768 rows of 4096: 195 us that way, 97 this way). 16-bit rows of single elements and the widest ones are loaded
+// directly.
 template <typename T, bool WIDE, int K, int N>
 struct RowsAhead {
   using Regs = RowRegs<T, WIDE, K>;
-  static constexpr int kElements = K * Regs::V, kBytes = 16 * K;
-  static constexpr bool kStaged = WIDE && kElements <= 32;
-  static constexpr int kDepth = !kStaged ? 1 : kElements <= 8 ? 4 : kElements * sizeof(T) <= 64 ? 2 : 1;
+  static constexpr int kElements = K * Regs::V, kPiece = WIDE ? 16 : 4, kBytes = kPiece * K;
+  static constexpr bool kStaged = (WIDE || sizeof(T) == 4) && kElements <= 32 && kElements * sizeof(T) * N <= 256;
+  static constexpr int kDepth = !kStaged ? 1 : kElements <= 8 ? 4 : kElements * sizeof(T) <= 32 ? 3 : kElements * sizeof(T) <= 64 && (kElements < 32 || N < 3) ? 2 : 1;
   uint32_t slot;  // of this thread, in the stage that comes next
   uint32_t first, last, stage;
 
   __device__ __forceinline__ explicit RowsAhead(void* shared) {
-    first = slot = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) + threadIdx.x * 16;
+    first = slot = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) + threadIdx.x * kPiece;
     stage = blockDim.x * kBytes * N;
     last = first + (kDepth - 1) * stage;
   }
@@ -173,9 +198,12 @@ struct RowsAhead {
     for (int k = 0; k < K; ++k) {
       const int c = (k * t.lanes + t.lane) * Regs::V;
       const bool ok = in && c < d;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + (n * K + k) * blockDim.x * 16),
-                   "l"(ok ? row + c * static_cast<int>(sizeof(T)) : row), "r"(ok ? 16 : 0), "f"(after)
-                   : "memory");
+      const uint32_t to = slot + (n * K + k) * blockDim.x * kPiece;
+      const char* from = ok ? row + c * static_cast<int>(sizeof(T)) : row;
+      if constexpr (WIDE)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0), "f"(after) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(ok ? 4 : 0), "f"(after) : "memory");
     }
   }
   __device__ __forceinline__ void next() {
@@ -189,8 +217,10 @@ struct RowsAhead {
       if constexpr (WIDE)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(r.raw[k].x), "=r"(r.raw[k].y), "=r"(r.raw[k].z), "=r"(r.raw[k].w)
-                     : "r"(slot + (n * K + k) * blockDim.x * 16)
+                     : "r"(slot + (n * K + k) * blockDim.x * kPiece)
                      : "memory");
+      else if constexpr (sizeof(T) == 4)
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r.raw[k]) : "r"(slot + (n * K + k) * blockDim.x * kPiece) : "memory");
   }
 };
 
@@ -287,12 +317,14 @@ __host__ __device__ constexpr int norm_threads_sm(bool backward, int values) { r
 __host__ __device__ constexpr int norm_threads_cta(bool backward, int values) { return values <= 8 && backward ? 256 : 512; }
 
 // The next rows are on their way while these are worked on.
-template <typename T, bool WIDE, int LANES, int K>
+template <typename T, bool WIDE, int LANES, int K, bool FLAT>
 __global__ void __launch_bounds__(norm_threads_cta(false, K * Piece<T, WIDE>::kElements), norm_threads_sm(false, K * Piece<T, WIDE>::kElements) / norm_threads_cta(false, K * Piece<T, WIDE>::kElements))
 fla_layer_norm_fwd_kernel(const LayerNormParams p) {
   using Regs = RowRegs<T, WIDE, K>;
   constexpr int V = Regs::V, P = Regs::kPairs;
-  __shared__ float parts[2][1][32];
+  // Two rows at a time share the latency of shuffles and barriers.
+  constexpr int kRows = RowsAhead<T, WIDE, K, 2>::kStaged && K * V <= 8 ? 2 : 1;
+  __shared__ float parts[2][kRows][32];
   int turn = 0;
   const RowTeam t = row_team<LANES>(p);
   const int head = blockIdx.y;
@@ -303,80 +335,97 @@ fla_layer_norm_fwd_kernel(const LayerNormParams p) {
   extern __shared__ uint4 slots[];
   using Ahead = RowsAhead<T, WIDE, K, 2>;
   Ahead ahead(slots);
-  Regs x, z;
+  constexpr int R = kRows;
+  Regs x[R], z[R];
   unsigned next = blockIdx.x * t.groups + t.group;
-  auto fetch = [&](float after) {  // the row after those that are on their way
+  Cursor<FLAT> x_at(p.x, head, next, stride), z_at(p.z, head, next, stride), s_at(p.s, head, next, stride), y_at(p.y, head, next, stride);
+  auto fetch = [&](int r, float after) {  // the row after those that are on their way
     const bool in = next < rows;
-    const char* xr = p.x.ptr + (in ? row_offset(p.x, p, next, head) : 0);
-    const char* zr = p.z.ptr + (in && p.z.ptr != nullptr ? row_offset(p.z, p, next, head) : 0);
+    const char *xr = x_at.get(p, next, in), *zr = z_at.get(p, next, in && p.z.ptr != nullptr);
     if constexpr (Ahead::kStaged) {
       ahead.start(0, xr, t, p.d, in, after);
       if (p.z.ptr != nullptr) ahead.start(1, zr, t, p.d, in, after);
       ahead.next();
     } else {
-      x.load(xr, t.lane, t.lanes, p.d, in);
-      if (p.z.ptr != nullptr) z.load(zr, t.lane, t.lanes, p.d, in);
+      x[r].load(xr, t.lane, t.lanes, p.d, in);
+      if (p.z.ptr != nullptr) z[r].load(zr, t.lane, t.lanes, p.d, in);
     }
+    x_at.advance();
+    z_at.advance();
     next += stride;
   };
 #pragma unroll
-  for (int s = 0; s < Ahead::kDepth; ++s) fetch(0.f);
+  for (int s = 0; s < Ahead::kDepth; ++s) fetch(0, 0.f);
   unsigned j = blockIdx.x * t.groups + t.group;
   // (every lane of a warp takes the same turns: its first row decides)
-  for (unsigned base = blockIdx.x * t.groups; base < rows; base += stride, j += stride) {
-    const bool in = j < rows;
-    if constexpr (Ahead::kStaged) {
-      ahead.arrived();
-      ahead.take(0, x);
-      if (p.z.ptr != nullptr) ahead.take(1, z);
-    }
-    float2 v[P];
-    if (p.z.ptr != nullptr) {
-      float2 more[P];
-      x.widen(v);
-      z.widen(more);
+  for (unsigned base = blockIdx.x * t.groups; base < rows; base += R * stride, j += R * stride) {
+    float2 v[R][P];
+    float sum[R];
 #pragma unroll
-      for (int i = 0; i < P; ++i) v[i] = add2(v[i], more[i]);
-      x.narrow(v);  // what is normalised is the sum as it is stored
-      x.store(p.s.ptr + (in ? row_offset(p.s, p, j, head) : 0), t.lane, t.lanes, p.d, in);
-    }
-    x.widen(v);
-    float2 pair = v[0];
-#pragma unroll
-    for (int i = 1; i < P; ++i) pair = add2(pair, v[i]);
-    float sum[1] = {pair.x + pair.y};
-    fetch(sum[0]);
-    sum_over_row<LANES>(sum, parts, turn, t);
-    const float mean = sum[0] * over_d;
-#pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = add2(v[i], both(-mean));
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        if ((2 * i / V * t.lanes + t.lane) * V >= p.d) v[i].x = 0.f;
-        if (((2 * i + 1) / V * t.lanes + t.lane) * V >= p.d) v[i].y = 0.f;
+    for (int r = 0; r < R; ++r) {
+      const unsigned row = j + r * stride;
+      if constexpr (Ahead::kStaged) {
+        ahead.arrived();
+        ahead.take(0, x[r]);
+        if (p.z.ptr != nullptr) ahead.take(1, z[r]);
       }
-    }
-    pair = mul2(v[0], v[0]);
+      if (p.z.ptr != nullptr) {
+        float2 more[P];
+        x[r].widen(v[r]);
+        z[r].widen(more);
 #pragma unroll
-    for (int i = 1; i < P; ++i) pair = fma2(v[i], v[i], pair);
-    sum[0] = pair.x + pair.y;
+        for (int i = 0; i < P; ++i) v[r][i] = add2(v[r][i], more[i]);
+        x[r].narrow(v[r]);  // what is normalised is the sum as it is stored
+        x[r].store(s_at.get(p, row, row < rows), t.lane, t.lanes, p.d, row < rows);
+        s_at.advance();
+      }
+      x[r].widen(v[r]);
+      float2 pair = v[r][0];
+#pragma unroll
+      for (int i = 1; i < P; ++i) pair = add2(pair, v[r][i]);
+      sum[r] = pair.x + pair.y;
+      fetch(r, sum[r]);
+    }
     sum_over_row<LANES>(sum, parts, turn, t);
-    const float r = reciprocal_root(fmaf(sum[0], over_d, p.eps));
-    if (p.stats != nullptr && t.lane == 0 && in)
-      *reinterpret_cast<float2*>(p.stats + 2 * (head * p.rows + j)) = make_float2(mean, r);
-    Regs y;
+    float mean[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = sum[r] * over_d;
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[r][i] = add2(v[r][i], both(-mean[r]));
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          if ((2 * i / V * t.lanes + t.lane) * V >= p.d) v[r][i].x = 0.f;
+          if (((2 * i + 1) / V * t.lanes + t.lane) * V >= p.d) v[r][i].y = 0.f;
+        }
+      }
+      float2 pair = mul2(v[r][0], v[r][0]);
+#pragma unroll
+      for (int i = 1; i < P; ++i) pair = fma2(v[r][i], v[r][i], pair);
+      sum[r] = pair.x + pair.y;
+    }
+    sum_over_row<LANES>(sum, parts, turn, t);
     float2 w[P], b[P];
     weight.get(w, t.lane, t.lanes, p.d);
     bias.get(b, t.lane, t.lanes, p.d);
 #pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = fma2(mul2(v[i], both(r)), w[i], b[i]);
-    y.narrow(v);
-    y.store(p.y.ptr + (in ? row_offset(p.y, p, j, head) : 0), t.lane, t.lanes, p.d, in);
+    for (int r = 0; r < R; ++r) {
+      const unsigned row = j + r * stride;
+      const float root = reciprocal_root(fmaf(sum[r], over_d, p.eps));
+      if (p.stats != nullptr && t.lane == 0 && row < rows)
+        *reinterpret_cast<float2*>(p.stats + 2 * (head * p.rows + row)) = make_float2(mean[r], root);
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[r][i] = fma2(mul2(v[r][i], both(root)), w[i], b[i]);
+      Regs y;
+      y.narrow(v[r]);
+      y.store(y_at.get(p, row, row < rows), t.lane, t.lanes, p.d, row < rows);
+      y_at.advance();
+    }
   }
 }
 
-template <typename T, bool WIDE, int LANES, int K>
+template <typename T, bool WIDE, int LANES, int K, bool FLAT>
 __global__ void __launch_bounds__(norm_threads_cta(true, K * Piece<T, WIDE>::kElements), norm_threads_sm(true, K * Piece<T, WIDE>::kElements) / norm_threads_cta(true, K * Piece<T, WIDE>::kElements))
 fla_layer_norm_bwd_kernel(const LayerNormParams p) {
   using Regs = RowRegs<T, WIDE, K>;
@@ -388,9 +437,11 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
   const unsigned rows = static_cast<unsigned>(p.rows), stride = gridDim.x * t.groups;
   const float over_d = 1.f / p.d;
   const LaneWeights<T, WIDE, K> weight(p.w, p.w_wide, 1.f, head, t.lane, t.lanes, p.d);
-  float2 dw[P], db[P];
+  // The sums for the weights: in registers, or, where 32 elements a thread leave none, in shared memory behind the rows.
+  constexpr bool kSumsShared = WIDE && K * V == 32;
+  float2 dw[kSumsShared ? 1 : P], db[kSumsShared ? 1 : P];
 #pragma unroll
-  for (int i = 0; i < P; ++i) dw[i] = db[i] = both(0.f);
+  for (int i = 0; i < (kSumsShared ? 1 : P); ++i) dw[i] = db[i] = both(0.f);
   extern __shared__ uint4 slots[];  // rows on their way; then [2][d] sums, where a CTA has several rows at a time
   using Ahead = RowsAhead<T, WIDE, K, 3>;
   Ahead ahead(slots);
@@ -398,25 +449,32 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
   float2 stats;
   const unsigned start = blockIdx.x * t.groups + t.group;
   unsigned next = start, stats_next = start;
+  Cursor<FLAT> x_at(p.x, head, start, stride), dy_at(p.dy, head, start, stride), ds_at(p.ds, head, start, stride), dx_at(p.dx, head, start, stride);
   auto fetch = [&](float after) {  // the row after those that are on their way
     const bool in = next < rows;
-    const char* xr = p.x.ptr + (in ? row_offset(p.x, p, next, head) : 0);
-    const char* gr = p.dy.ptr + (in ? row_offset(p.dy, p, next, head) : 0);
+    const char *xr = x_at.get(p, next, in), *gr = dy_at.get(p, next, in);
     if constexpr (Ahead::kStaged) {
       ahead.start(0, xr, t, p.d, in, after);
       ahead.start(1, gr, t, p.d, in, after);
-      if (p.ds.ptr != nullptr) ahead.start(2, p.ds.ptr + (in ? row_offset(p.ds, p, next, head) : 0), t, p.d, in, after);
+      if (p.ds.ptr != nullptr) ahead.start(2, ds_at.get(p, next, in), t, p.d, in, after);
+      ds_at.advance();
       ahead.next();
     } else {
       x.load(xr, t.lane, t.lanes, p.d, in);
       dy.load(gr, t.lane, t.lanes, p.d, in);
     }
+    x_at.advance();
+    dy_at.advance();
     next += stride;
   };
   auto fetch_stats = [&] {
     stats = stats_next < rows ? __ldg(reinterpret_cast<const float2*>(p.stats + 2 * (head * p.rows + stats_next))) : both(0.f);
     stats_next += stride;
   };
+  float2* const sums_at = reinterpret_cast<float2*>(reinterpret_cast<char*>(slots) + (Ahead::kStaged ? 3 * Ahead::kDepth * Ahead::kBytes * blockDim.x : 0)) + threadIdx.x;
+  if constexpr (kSumsShared)
+#pragma unroll
+    for (int i = 0; i < 2 * P; ++i) sums_at[i * blockDim.x] = both(0.f);
   fetch_stats();
 #pragma unroll
   for (int s = 0; s < Ahead::kDepth; ++s) fetch(0.f);
@@ -429,7 +487,8 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
       ahead.take(1, dy);
       if (p.ds.ptr != nullptr) ahead.take(2, ds);
     } else {
-      if (p.ds.ptr != nullptr) ds.load(p.ds.ptr + (in ? row_offset(p.ds, p, j, head) : 0), t.lane, t.lanes, p.d, in);
+      if (p.ds.ptr != nullptr) ds.load(ds_at.get(p, j, in), t.lane, t.lanes, p.d, in);
+      ds_at.advance();
     }
     const float r = stats.y;
     const float2 shift = both(-stats.x);
@@ -443,8 +502,14 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       n[i] = mul2(add2(n[i], shift), both(r));
-      dw[i] = fma2(u[i], n[i], dw[i]);
-      db[i] = add2(db[i], u[i]);
+      if constexpr (kSumsShared) {
+        float2* const at = sums_at + 2 * i * blockDim.x;
+        at[0] = fma2(u[i], n[i], at[0]);
+        at[blockDim.x] = add2(at[blockDim.x], u[i]);
+      } else {
+        dw[i] = fma2(u[i], n[i], dw[i]);
+        db[i] = add2(db[i], u[i]);
+      }
       u[i] = mul2(u[i], w[i]);
       s0 = add2(s0, u[i]);
       s1 = fma2(u[i], n[i], s1);
@@ -463,11 +528,25 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
     }
     Regs dx;
     dx.narrow(u);
-    dx.store(p.dx.ptr + (in ? row_offset(p.dx, p, j, head) : 0), t.lane, t.lanes, p.d, in);
+    dx.store(dx_at.get(p, j, in), t.lane, t.lanes, p.d, in);
+    dx_at.advance();
   }
   if (p.parts == nullptr) return;
+  asm volatile("griddepcontrol.launch_dependents;");  // (the kernel that joins the CTAs' sums may be set up)
   float* out = p.parts + (static_cast<long long>(blockIdx.x) * 2 * p.heads + head) * p.d;  // dw; db lies heads * d behind
   const long long db_at = static_cast<long long>(p.heads) * p.d;
+  if constexpr (kSumsShared) {  // (one row at a time: every thread has columns of its own)
+#pragma unroll
+    for (int e = 0; e < 2 * P; ++e) {
+      const int c = (e / V * t.lanes + t.lane) * V + e % V;
+      const float2 ew = sums_at[2 * (e / 2) * blockDim.x], eb = sums_at[(2 * (e / 2) + 1) * blockDim.x];
+      if (c < p.d) {
+        out[c] = e % 2 ? ew.y : ew.x;
+        out[db_at + c] = e % 2 ? eb.y : eb.x;
+      }
+    }
+    return;
+  } else {
   // The groups of a warp join by shuffles, then warps or groups of warps one after the other.
   constexpr int kSpan = LANES ? 32 : 0;
   float* const joined = reinterpret_cast<float*>(slots);
@@ -503,6 +582,7 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
       out[c] = joined[c];
       out[db_at + c] = joined[p.d + c];
     }
+  }
 }
 
 // dw and db from the CTAs' sums: 32 columns a block, 32 shares of the CTAs side by side, joined in order.
@@ -511,12 +591,15 @@ __global__ void __launch_bounds__(1024) fla_layer_norm_weights_kernel(const floa
   __shared__ float shares[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x, share = threadIdx.y;
   W* out = blockIdx.y ? db : dw;
-  if (out == nullptr) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float sum = 0.f;
-  if (c < columns) {
-    const float* at = parts + static_cast<long long>(blockIdx.y) * columns + c;
-#pragma unroll 4
-    for (int i = share; i < ctas; i += 32) sum += __ldg(at + static_cast<long long>(i) * 2 * columns);
+  const float* at = parts + static_cast<long long>(blockIdx.y) * columns + c;
+  for (int i = share; i < ctas && c < columns; i += 32 * 8) {
+    float some[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) some[k] = i + 32 * k < ctas ? __ldcg(at + static_cast<long long>(i + 32 * k) * 2 * columns) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += some[k];
   }
   shares[share][threadIdx.x] = sum;
   __syncthreads();
@@ -525,7 +608,7 @@ __global__ void __launch_bounds__(1024) fla_layer_norm_weights_kernel(const floa
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const int mine = blockIdx.x * 32 + share;
-  if (threadIdx.x == 0 && mine < columns) {
+  if (threadIdx.x == 0 && mine < columns && out != nullptr) {
     if constexpr (sizeof(W) == 4) out[mine] = sum;
     else out[mine] = static_cast<W>(sum);
   }
@@ -547,6 +630,7 @@ struct NormPlan {
   bool wide;
   int lanes, k;       // lanes: 0 where a row has whole warps, p.lanes threads
   int threads, ctas;  // ctas: of a head
+  bool flat;
 };
 
 NormRows norm_rows(const FlaTensor& t, int size, bool heads_apart) {
@@ -582,8 +666,27 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
   p.d = a->dim;
   p.eps = a->eps;
   NormRows* const used[] = {&p.x, backward ? &p.dy : &p.y, backward ? &p.dx : &p.s, backward ? &p.ds : &p.z};
-  // neighbouring dims that are one in every tensor
   long long n0 = a->batch;
+  // Rows are numbered as they lie in memory in what is normalised (the same tensor in both passes, whatever the others
+  // look like: `stats` goes by these numbers).
+  const NormRows order = backward || p.s.ptr == nullptr ? p.x : p.s;
+  auto swap01 = [&] {
+    for (NormRows* t : used) std::swap(t->s0, t->s1);
+    const int n = static_cast<int>(n0);
+    n0 = p.n1;
+    p.n1 = n;
+  };
+  auto swap12 = [&] {
+    for (NormRows* t : used) std::swap(t->s1, t->s2);
+    std::swap(p.n1, p.n2);
+  };
+  {
+    long long s0 = n0 == 1 ? 0 : order.s0, s1 = p.n1 == 1 ? 0 : order.s1, s2 = p.n2 == 1 ? 0 : order.s2;
+    if (s1 > s0) swap01(), std::swap(s0, s1);
+    if (s2 > s1) swap12(), std::swap(s1, s2);
+    if (s1 > s0) swap01();
+  }
+  // neighbouring dims that are one in every tensor
   auto every = [&](auto&& holds) {
     for (NormRows* t : used)
       if (t->ptr != nullptr && !holds(*t)) return false;
@@ -610,19 +713,19 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
     for (NormRows* t : used) t->s1 = t->s0;
   }
   const int per = 16 / size;
+  plan.flat = p.n1 == 1 && p.rows == p.n2;
   auto aligned = [](const void* q, int n) { return reinterpret_cast<uintptr_t>(q) % n == 0; };
   plan.wide = p.d % per == 0 && aligned(p.w, 16) && aligned(p.b, 16) && every([&](const NormRows& t) {
                 return aligned(t.ptr, 16) && (p.heads == 1 || t.sh % 16 == 0) && (n0 == 1 || t.s0 % 16 == 0) &&
                        (p.n1 == 1 || t.s1 % 16 == 0) && (p.n2 == 1 || t.s2 % 16 == 0);
               });
-  // A thread holds up to 8 elements of a row, backward of rows above 1024 columns 16; 16, 32 or 64 of the widest.
+  // A thread holds up to 16 elements of a row, 8 of the narrowest and 32 or 64 of the widest.
   const int pieces = plan.wide ? p.d / per : p.d;
   const int held = plan.wide ? per : 1;
-  const int values = p.d <= (backward ? 1024 : 4096) ? 8 : p.d <= 8192 ? 16 : p.d <= 16384 ? 32 : 64;
+  const int values = p.d <= 32 ? 8 : p.d <= 8192 ? 16 : p.d <= 16384 ? 32 : 64;
   plan.k = values / held;
-  if (plan.wide && pieces <= 32) plan.k = 1;
-  if (!plan.wide && pieces <= 128) plan.k = pieces <= 64 ? 2 : 4;
-  plan.lanes = plan.wide && pieces <= 8 ? 8 : plan.wide && pieces <= 16 ? 16 : pieces <= 32 * plan.k ? 32 : 0;
+  if (!plan.wide) plan.k = p.d <= 64 ? 2 : p.d <= 128 ? 4 : p.d <= 256 ? 8 : plan.k;
+  plan.lanes = plan.wide && pieces <= 4 * plan.k ? 4 : plan.wide && pieces <= 8 * plan.k ? 8 : plan.wide && pieces <= 16 * plan.k ? 16 : pieces <= 32 * plan.k ? 32 : 0;
   p.lanes = plan.lanes ? plan.lanes : (pieces + plan.k * 32 - 1) / (plan.k * 32) * 32;
   const long long groups = std::max(1, 256 / p.lanes);
   plan.threads = static_cast<int>(groups) * p.lanes;
@@ -636,14 +739,19 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
 
 size_t norm_workspace(const NormPlan& plan) { return static_cast<size_t>(plan.ctas) * 2 * plan.p.heads * plan.p.d * sizeof(float); }
 
-template <typename T, bool WIDE, int LANES, int K>
-int norm_launch(const NormPlan& plan, bool backward, cudaStream_t stream) {
-  using Ahead = fla::RowsAhead<T, WIDE, K, 1>;
+template <typename T, bool WIDE, int LANES, int K, bool FLAT>
+int norm_launch_kernel(const NormPlan& plan, bool backward, cudaStream_t stream) {
+  using Forward = fla::RowsAhead<T, WIDE, K, 2>;
+  using Backward = fla::RowsAhead<T, WIDE, K, 3>;
   const dim3 grid(plan.ctas, plan.p.heads);
-  const auto kernel = backward ? fla::fla_layer_norm_bwd_kernel<T, WIDE, LANES, K> : fla::fla_layer_norm_fwd_kernel<T, WIDE, LANES, K>;
+  const auto kernel = backward ? fla::fla_layer_norm_bwd_kernel<T, WIDE, LANES, K, FLAT>
+                               : fla::fla_layer_norm_fwd_kernel<T, WIDE, LANES, K, FLAT>;
   // (the stages are laid out for the most tensors that a row can have)
-  size_t shared = Ahead::kStaged ? static_cast<size_t>(Ahead::kDepth) * Ahead::kBytes * plan.threads * (backward ? 3 : 2) : 0;
-  if (backward && plan.p.parts != nullptr && plan.threads > std::max(32, plan.p.lanes))
+  size_t shared = static_cast<size_t>(plan.threads) * (backward ? Backward::kStaged * Backward::kDepth * Backward::kBytes * 3
+                                                                : Forward::kStaged * Forward::kDepth * Forward::kBytes * 2);
+  constexpr int kElements = Backward::kElements;
+  if (backward && WIDE && kElements == 32) shared += 2 * kElements * plan.threads * sizeof(float);
+  else if (backward && plan.p.parts != nullptr && plan.threads > std::max(32, plan.p.lanes))
     shared = std::max(shared, 2 * plan.p.d * sizeof(float));
   if (shared > 40 * 1024 &&  // (48 KB go without, with what the kernels declare)
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess)
@@ -652,24 +760,29 @@ int norm_launch(const NormPlan& plan, bool backward, cudaStream_t stream) {
   return fla::launched(cudaSuccess, backward ? "fla_layer_norm_bwd_kernel" : "fla_layer_norm_fwd_kernel");
 }
 
+template <typename T, bool WIDE, int LANES, int K>
+int norm_launch(const NormPlan& plan, bool backward, cudaStream_t stream) {
+  return plan.flat ? norm_launch_kernel<T, WIDE, LANES, K, true>(plan, backward, stream)
+                   : norm_launch_kernel<T, WIDE, LANES, K, false>(plan, backward, stream);
+}
+
 template <typename T>
 int norm_launch_type(const NormPlan& plan, bool backward, cudaStream_t stream) {
   constexpr int kPer = 16 / sizeof(T), k8 = 8 / kPer;  // elements of a piece, pieces of 8 elements
   if (plan.wide) {
-    if (plan.lanes == 8) return norm_launch<T, true, 8, 1>(plan, backward, stream);
-    if (plan.lanes == 16) return norm_launch<T, true, 16, 1>(plan, backward, stream);
-    if (plan.lanes == 32 && plan.k == 1) return norm_launch<T, true, 32, 1>(plan, backward, stream);
-    if constexpr (k8 > 1)
-      if (plan.lanes == 32) return norm_launch<T, true, 32, k8>(plan, backward, stream);
-    if (plan.k == k8) return norm_launch<T, true, 0, k8>(plan, backward, stream);
+    if (plan.k == k8) return norm_launch<T, true, 4, k8>(plan, backward, stream);
+    if (plan.lanes == 4) return norm_launch<T, true, 4, 2 * k8>(plan, backward, stream);
+    if (plan.lanes == 8) return norm_launch<T, true, 8, 2 * k8>(plan, backward, stream);
+    if (plan.lanes == 16) return norm_launch<T, true, 16, 2 * k8>(plan, backward, stream);
+    if (plan.lanes == 32) return norm_launch<T, true, 32, 2 * k8>(plan, backward, stream);
     if (plan.k == 2 * k8) return norm_launch<T, true, 0, 2 * k8>(plan, backward, stream);
     if (plan.k == 4 * k8) return norm_launch<T, true, 0, 4 * k8>(plan, backward, stream);
     return norm_launch<T, true, 0, 8 * k8>(plan, backward, stream);
   }
   if (plan.lanes && plan.k == 2) return norm_launch<T, false, 32, 2>(plan, backward, stream);
   if (plan.lanes && plan.k == 4) return norm_launch<T, false, 32, 4>(plan, backward, stream);
-  if (plan.lanes) return norm_launch<T, false, 32, 8>(plan, backward, stream);
-  if (plan.k == 8) return norm_launch<T, false, 0, 8>(plan, backward, stream);
+  if (plan.lanes && plan.k == 8) return norm_launch<T, false, 32, 8>(plan, backward, stream);
+  if (plan.lanes) return norm_launch<T, false, 32, 16>(plan, backward, stream);
   if (plan.k == 16) return norm_launch<T, false, 0, 16>(plan, backward, stream);
   if (plan.k == 32) return norm_launch<T, false, 0, 32>(plan, backward, stream);
   return norm_launch<T, false, 0, 64>(plan, backward, stream);
@@ -736,19 +849,25 @@ int fla_sm100_layer_norm_bwd(const FlaLayerNormArgs* a) {
   if (const int rc = norm_dispatch(a, plan, true)) return rc;
   if (!weights) return FLA_OK;
   const int columns = plan.p.heads * plan.p.d;
-  const dim3 grid((columns + 31) / 32, 2);
-  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
-  if (a->w_dtype == FLA_DTYPE_F32)
-    fla::fla_layer_norm_weights_kernel<<<grid, dim3(32, 32), 0, stream>>>(plan.p.parts, plan.ctas, columns, static_cast<float*>(a->d_weight),
-                                                                static_cast<float*>(a->d_bias));
-  else if (a->w_dtype == FLA_DTYPE_F16)
-    fla::fla_layer_norm_weights_kernel<<<grid, dim3(32, 32), 0, stream>>>(plan.p.parts, plan.ctas, columns, static_cast<__half*>(a->d_weight),
-                                                                static_cast<__half*>(a->d_bias));
-  else
-    fla::fla_layer_norm_weights_kernel<<<grid, dim3(32, 32), 0, stream>>>(plan.p.parts, plan.ctas, columns,
-                                                                static_cast<__nv_bfloat16*>(a->d_weight),
-                                                                static_cast<__nv_bfloat16*>(a->d_bias));
-  return fla::launched(cudaSuccess, "fla_layer_norm_weights_kernel");
+  // Set up while the first kernel runs; it waits for that one's end (which is a launch's latency less, 3 us).
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((columns + 31) / 32, 2);
+  cfg.blockDim = dim3(32, 32);
+  cfg.stream = static_cast<cudaStream_t>(a->stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  auto go = [&](auto* zero) {
+    using W = std::remove_pointer_t<decltype(zero)>;
+    return fla::launched(cudaLaunchKernelEx(&cfg, fla::fla_layer_norm_weights_kernel<W>, static_cast<const float*>(plan.p.parts), plan.ctas,
+                                            columns, static_cast<W*>(a->d_weight), static_cast<W*>(a->d_bias)),
+                         "fla_layer_norm_weights_kernel");
+  };
+  if (a->w_dtype == FLA_DTYPE_F32) return go(static_cast<float*>(nullptr));
+  if (a->w_dtype == FLA_DTYPE_F16) return go(static_cast<__half*>(nullptr));
+  return go(static_cast<__nv_bfloat16*>(nullptr));
 }
 
 }  // extern "C"
