@@ -472,7 +472,7 @@ struct InMemory {
 };
 
 template <typename TX, typename TG, bool PAIR, int LPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_fwd_kernel(const RecurrenceParams p) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_direct_fwd_kernel(const RecurrenceParams p) {
   constexpr int T = kRunTokens<TX, TG>;
   __shared__ RecurrenceShared<LPR, THREADS> sh;
   Team team;
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_fwd_ke
 }
 
 template <typename TX, typename TG, bool PAIR, int LPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_kernel(const RecurrenceParams p) {
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_bwd_kernel(const RecurrenceParams p) {
   constexpr int T = kRunTokens<TX, TG>;
   __shared__ RecurrenceShared<LPR, THREADS> sh;
   Team team;
@@ -671,6 +671,282 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_ker
   if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
 }
 
+// ------------------------------------------------------------------------------------------------------------
+// The same with rows that lie on 16-byte boundaries: a warp brings the rows of its runs of the next steps into a tile of its
+// own in shared memory, 16 bytes a lane and asynchronously, takes them into registers, and lets results leave the same
+// way. The loads of a step so are on their way through the whole step before, its exchange included, and there are a
+// quarter as many of them.
+
+// T-typed rows of the runs of a warp: TOK tokens each, 2 LPR columns.
+template <typename T, int LPR, int TOK>
+struct WarpTile {
+  static constexpr int kRow = 2 * LPR * sizeof(T), kPieces = kRow / 16, kRows = TOK * (32 / LPR);
+  static constexpr int kBytes = kRows * kRow, kEach = kBytes / 512, kRowsEach = 32 / kPieces;
+  char* base;                // of the batch entry, head and tile of channels
+  uint32_t at, row, first;   // bytes; the lane's first row of the warp's
+  bool in;                   // its piece lies inside the row
+
+  __device__ __forceinline__ WarpTile(const RecurrenceTensor& t, const Place& w, int tile_column, int columns, int first_token) {
+    base = static_cast<char*>(t.ptr) + (w.b * t.sb + w.h * t.sh + tile_column) * static_cast<long long>(sizeof(T));
+    row = static_cast<uint32_t>(t.sn) * sizeof(T);
+    const int lane = threadIdx.x % 32, piece = lane % kPieces;
+    first = lane / kPieces;
+    at = (first_token + first) * row + piece * 16;
+    in = piece * 16 < columns * static_cast<int>(sizeof(T));
+  }
+  __device__ __forceinline__ char* step(const RecurrenceTensor& t, long long token) const {
+    return base + token * t.sn * static_cast<long long>(sizeof(T));
+  }
+  // Rows past the last token (`left`: how many of the warp's rows there are) are zero, the identity.
+  __device__ __forceinline__ void copy(uint32_t tile, const char* step, int left) const {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const bool ok = in && static_cast<int>(first) + k * kRowsEach < left;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + (k * 32 + threadIdx.x % 32) * 16),
+                   "l"(ok ? step + (at + k * kRowsEach * row) : base), "r"(ok ? 16 : 0)
+                   : "memory");
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t tile, char* step, int left) const {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      uint4 v;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(tile + (k * 32 + threadIdx.x % 32) * 16)
+                   : "memory");
+      if (in && static_cast<int>(first) + k * kRowsEach < left) *reinterpret_cast<uint4*>(step + (at + k * kRowsEach * row)) = v;
+    }
+  }
+  // A token's two channels of a thread, whose run's rows begin at `run`.
+  __device__ __forceinline__ static typename PairOf<T>::Raw get(uint32_t run, int t) {
+    typename PairOf<T>::Raw r;
+    if constexpr (sizeof(T) == 4)
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(run + t * kRow) : "memory");
+    else
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(run + t * kRow) : "memory");
+    return r;
+  }
+  __device__ __forceinline__ static void put(uint32_t run, int t, float2 v) {
+    const auto r = pack_pair<T>(v);
+    if constexpr (sizeof(T) == 4)
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(run + t * kRow), "f"(r.x), "f"(r.y) : "memory");
+    else
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(run + t * kRow), "r"(r) : "memory");
+  }
+};
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  __syncwarp();
+}
+
+constexpr int kFwdStages = 2;
+template <typename TX, typename TG, int LPR>
+constexpr int kFwdWarpBytes = kFwdStages * (WarpTile<TX, LPR, kRunTokens<TX, TG>>::kBytes + WarpTile<TG, LPR, kRunTokens<TX, TG>>::kBytes) +
+                              WarpTile<TX, LPR, kRunTokens<TX, TG>>::kBytes;
+template <typename TX, typename TG, int LPR>
+constexpr int kBwdWarpBytes = 3 * WarpTile<TX, LPR, kRunTokens<TX, TG>>::kBytes + 2 * WarpTile<TG, LPR, kRunTokens<TX, TG>>::kBytes;
+
+template <typename TX, typename TG, int LPR, int THREADS>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_fwd_kernel(const RecurrenceParams p) {
+  constexpr int T = kRunTokens<TX, TG>, kRuns = THREADS / LPR;
+  using TileX = WarpTile<TX, LPR, T>;
+  using TileG = WarpTile<TG, LPR, T>;
+  extern __shared__ uint4 tiles[];
+  __shared__ RecurrenceShared<LPR, THREADS> sh;
+  Team team;
+  Place w;
+  take_place<true>(p, sh, &team, &w);
+  bool lost = false;
+  const int column = w.c0 - 2 * team.lane;  // of the tile
+  const int first = (team.rank * kRuns + team.run / (32 / LPR) * (32 / LPR)) * T;  // of the warp's tokens, in the step
+  const int mine = team.run % (32 / LPR) * T;                                      // of the run's, among them
+  const TileX xt(p.x, w, column, p.c - column, first), ot(p.o, w, column, p.c - column, first);
+  const TileG gt(p.g, w, column, p.c - column, first);
+  const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kFwdWarpBytes<TX, TG, LPR>;
+  const uint32_t out = space + kFwdStages * (TileX::kBytes + TileG::kBytes);
+  const uint32_t x_run = mine * TileX::kRow + team.lane * 2 * sizeof(TX), g_run = mine * TileG::kRow + team.lane * 2 * sizeof(TG);
+  const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
+  float2 carry = make_float2(0.f, 0.f);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, true>(p.start + cell, 1, w.ok0, w.ok1);
+
+  const int span = team.ranks * kRuns * T;  // tokens a step
+  const int steps = (p.n - 1) / span + 1, runs_all = (p.n - 1) / T + 1;
+  auto bring = [&](int step) {
+    const uint32_t slot = space + step % kFwdStages * (TileX::kBytes + TileG::kBytes);
+    const long long token = static_cast<long long>(step) * span;
+    const int left = step < steps ? p.n - step * span - first : 0;
+    xt.copy(slot, xt.step(p.x, token), left);
+    gt.copy(slot + TileX::kBytes, gt.step(p.g, token), left);
+    copies_end();
+  };
+#pragma unroll
+  for (int s = 0; s < kFwdStages; ++s) bring(s);
+  if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
+  for (int step = 0; step < steps; ++step) {
+    const uint32_t slot = space + step % kFwdStages * (TileX::kBytes + TileG::kBytes);
+    typename PairOf<TX>::Raw x[T];
+    typename PairOf<TG>::Raw g[T];
+    copies_wait<kFwdStages - 1>();
+    float2 sum = make_float2(0.f, 0.f), h = sum;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      x[t] = TileX::get(slot + x_run, t);
+      g[t] = TileG::get(slot + TileX::kBytes + g_run, t);
+      const float2 gv = unpack_pair<TG>(g[t]);
+      sum = add2(sum, gv);
+      h = advance<TX, false>(gv, h, unpack_pair<TX>(x[t]));
+    }
+    __syncwarp();  // every lane has its rows: the tile is free
+    bring(step + kFwdStages);
+    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    if (drops) {
+      const InMemory<typename PairOf<TX>::Raw, T> xm(x);
+      const InMemory<typename PairOf<TG>::Raw, T> gm(g);
+      h = advance_from<TX, TG, T>(make_float2(0.f, 0.f), xm.v, gm.v, nullptr);
+    }
+    h = exchange(sh, step, sum, h, team, p, carry, lost);
+    const int t0 = step * span + first + mine;
+    if (p.states != nullptr && t0 < p.n)
+      store_pair<float, true>(p.states + state_of(p, w, t0 / T, runs_all), 1, w.ok0, w.ok1, h);
+    anew(x);
+    anew(g);
+    if (!drops) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+        TileX::put(out + x_run, t, h);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        h = advance<TX, true>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+        TileX::put(out + x_run, t, h);
+      }
+    }
+    __syncwarp();
+    ot.store(out, ot.step(p.o, static_cast<long long>(step) * span), p.n - step * span - first);
+    __syncwarp();
+  }
+  if (p.end != nullptr && team.run == 0 && team.rank == 0) store_pair<float, true>(p.end + cell, 1, w.ok0, w.ok1, carry);
+  if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
+}
+
+template <typename TX, typename TG, int LPR, int THREADS>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_kernel(const RecurrenceParams p) {
+  constexpr int T = kRunTokens<TX, TG>, kRuns = THREADS / LPR, kWarpRuns = 32 / LPR;
+  using TileX = WarpTile<TX, LPR, T>;
+  using TileG = WarpTile<TG, LPR, T>;
+  extern __shared__ uint4 tiles[];
+  __shared__ RecurrenceShared<LPR, THREADS> sh;
+  Team team;
+  Place w;
+  take_place<true>(p, sh, &team, &w);
+  bool lost = false;
+  const int column = w.c0 - 2 * team.lane;
+  const int span = team.ranks * kRuns;                        // runs a step
+  const int nth = span - 1 - (team.rank * kRuns + team.run);  // of the step's runs, in the order of the tokens
+  const int first = nth / kWarpRuns * kWarpRuns * T, mine = nth % kWarpRuns * T;
+  const TileX xt(p.x, w, column, p.c - column, first), yt(p.o, w, column, p.o.ptr != nullptr ? p.c - column : 0, first);
+  const TileX dxt(p.dx, w, column, p.dx.ptr != nullptr ? p.c - column : 0, first);
+  const TileG gt(p.g, w, column, p.c - column, first), dgt(p.dg, w, column, p.dg.ptr != nullptr ? p.c - column : 0, first);
+  const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kBwdWarpBytes<TX, TG, LPR>;
+  const uint32_t y_at = space + TileX::kBytes, dx_at = space + 2 * TileX::kBytes, g_at = space + 3 * TileX::kBytes, dg_at = g_at + TileG::kBytes;
+  const uint32_t x_run = mine * TileX::kRow + team.lane * 2 * sizeof(TX), g_run = mine * TileG::kRow + team.lane * 2 * sizeof(TG);
+  const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
+  float2 carry = make_float2(0.f, 0.f);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, true>(p.start + cell, 1, w.ok0, w.ok1);
+
+  const int runs_all = (p.n - 1) / T + 1;
+  const int steps = (runs_all - 1) / span + 1;
+  float2 state;
+  // (a tensor that is not there copies nothing: its rows are zero)
+  const RecurrenceTensor& dy = p.o.ptr != nullptr ? p.o : p.x;
+  auto bring = [&](int step) {
+    const long long token = static_cast<long long>(step) * span * T;
+    const int left = step >= 0 ? static_cast<int>(p.n - token) - first : 0;
+    xt.copy(space, xt.step(p.x, token), left);
+    yt.copy(y_at, yt.step(dy, token), left);
+    gt.copy(g_at, gt.step(p.g, token), left);
+    copies_end();
+    state = make_float2(0.f, 0.f);
+    const int run = step * span + nth;
+    if (step >= 0 && run < runs_all) state = load_pair<float, true>(p.states + state_of(p, w, run, runs_all), 1, w.ok0, w.ok1);
+  };
+  bring(steps - 1);
+  if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
+  // The walk starts at the end; the runs behind the last token are the identity.
+  for (int step = steps - 1; step >= 0; --step) {
+    typename PairOf<TX>::Raw x[T], y[T];
+    typename PairOf<TG>::Raw g[T];
+    copies_wait<0>();
+    float2 sum = make_float2(0.f, 0.f), r = sum, h = state;
+#pragma unroll
+    for (int t = T - 1; t >= 0; --t) {
+      y[t] = TileX::get(y_at + x_run, t);
+      g[t] = TileG::get(g_at + g_run, t);
+      const float2 gv = unpack_pair<TG>(g[t]);
+      sum = add2(sum, gv);
+      r = retreat<TX, false>(gv, add2(unpack_pair<TX>(y[t]), r));
+    }
+    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    float2 before[T];  // the state before each token
+    anew(g);
+#pragma unroll
+    for (int t = 0; t < T; ++t) x[t] = TileX::get(space + x_run, t);
+    if (drops) {
+      const InMemory<typename PairOf<TX>::Raw, T> xm(x), ym(y);
+      const InMemory<typename PairOf<TG>::Raw, T> gm(g);
+      float2 bm[T];
+      r = retreat_from_zero<TX, TG, T>(ym.v, gm.v);
+      advance_from<TX, TG, T>(h, xm.v, gm.v, bm);
+#pragma unroll
+      for (int t = 0; t < T; ++t) before[t] = bm[t];
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        before[t] = h;
+        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+      }
+    }
+    __syncwarp();  // every lane has its rows: the tiles are free
+    bring(step - 1);
+    r = exchange(sh, steps - 1 - step, sum, r, team, p, carry, lost);
+    anew(y);
+    anew(g);
+    if (!drops) {
+#pragma unroll
+      for (int t = T - 1; t >= 0; --t) {
+        const float2 all = add2(unpack_pair<TX>(y[t]), r);
+        TileX::put(dx_at + x_run, t, all);
+        r = retreat<TX, false>(unpack_pair<TG>(g[t]), all);
+        TileG::put(dg_at + g_run, t, mul2(r, before[t]));
+      }
+    } else {
+#pragma unroll
+      for (int t = T - 1; t >= 0; --t) {
+        const float2 gv = unpack_pair<TG>(g[t]), all = add2(unpack_pair<TX>(y[t]), r);
+        TileX::put(dx_at + x_run, t, all);
+        r = retreat<TX, true>(gv, all);
+        float2 d = mul2(r, before[t]);
+        if (gv.x == -INFINITY) d.x = 0.f;
+        if (gv.y == -INFINITY) d.y = 0.f;
+        TileG::put(dg_at + g_run, t, d);
+      }
+    }
+    __syncwarp();
+    const long long token = static_cast<long long>(step) * span * T;
+    const int left = static_cast<int>(p.n - token) - first;
+    dxt.store(dx_at, dxt.step(p.dx, token), left);
+    dgt.store(dg_at, dgt.step(p.dg, token), left);
+    __syncwarp();
+  }
+  if (p.end != nullptr && team.run == 0 && team.rank == 0) store_pair<float, true>(p.end + cell, 1, w.ok0, w.ok1, carry);
+  if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
+}
+
 }  // namespace fla
 
 namespace {
@@ -686,7 +962,7 @@ int element_bytes(int dtype) { return dtype == FLA_DTYPE_F32 ? 4 : 2; }
 // other in every tensor are one row: narrow heads then fill a warp.
 struct Plan {
   RecurrenceParams p;
-  bool pair;
+  bool pair, wide;  // rows lie on boundaries of two elements, of 16 bytes
   int lpr;
   int batch;
   long long farthest;  // bytes from one token to the next, of the tensor where they are most
@@ -745,6 +1021,10 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
                 return reinterpret_cast<uintptr_t>(t.ptr) % (2 * size) == 0 && (p.n == 1 || t.sn % 2 == 0) &&
                        (p.heads == 1 || t.sh % 2 == 0) && (plan.batch == 1 || t.sb % 2 == 0);
               });
+  plan.wide = plan.pair && p.c * sizes[0] % 16 == 0 && p.c * sizes[1] % 16 == 0 && every([&](const RecurrenceTensor& t, int size) {
+                return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && (p.n == 1 || t.sn * size % 16 == 0) &&
+                       (p.heads == 1 || t.sh * size % 16 == 0) && (plan.batch == 1 || t.sb * size % 16 == 0);
+              });
   plan.farthest = 1;
   every([&](const RecurrenceTensor& t, int size) {
     plan.farthest = std::max(plan.farthest, t.sn * size);
@@ -773,7 +1053,7 @@ Shape shape_of(const Plan& plan, int run_tokens, int most_threads, int sm_count)
 template <typename TX, typename TG, bool PAIR, int LPR>
 int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
   constexpr int T = fla::kRunTokens<TX, TG>;
-  Shape shape = shape_of(plan, T, backward ? 512 : 1024, sm_count);
+  Shape shape = shape_of(plan, T, backward || plan.wide ? 512 : 1024, sm_count);
   const bool alone = plan.p.n <= kShortTokens || plan.farthest > 0x7fffffffLL / (shape.ranks * (shape.threads / LPR) * T);
   long long blocks = plan.p.tiles_all * shape.ranks;
   if (alone) {
@@ -791,15 +1071,30 @@ int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = shape.ranks > 1 ? 1 : 0;
-  auto go = [&](auto kernel, const char* name) { return fla::launched(cudaLaunchKernelEx(&cfg, kernel, plan.p), name); };
+  auto go = [&](auto kernel, const char* name) {
+    if (cfg.dynamicSmemBytes > 0 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         static_cast<int>(cfg.dynamicSmemBytes)) != cudaSuccess)
+      return static_cast<int>(FLA_ERR_CUDA);
+    return fla::launched(cudaLaunchKernelEx(&cfg, kernel, plan.p), name);
+  };
   if (alone)
     return backward ? go(fla::fla_recurrence_short_bwd_kernel<TX, TG, PAIR, LPR>, "fla_recurrence_short_bwd_kernel")
                     : go(fla::fla_recurrence_short_fwd_kernel<TX, TG, PAIR, LPR>, "fla_recurrence_short_fwd_kernel");
+  if constexpr (PAIR) {
+    if (plan.wide) {
+      cfg.dynamicSmemBytes = shape.threads / 32 * (backward ? fla::kBwdWarpBytes<TX, TG, LPR> : fla::kFwdWarpBytes<TX, TG, LPR>);
+      if (shape.threads == 256)
+        return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 256>, "fla_recurrence_bwd_kernel")
+                        : go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 256>, "fla_recurrence_fwd_kernel");
+      return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 512>, "fla_recurrence_bwd_kernel")
+                      : go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 512>, "fla_recurrence_fwd_kernel");
+    }
+  }
   if (shape.threads == 256)
-    return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_bwd_kernel")
-                    : go(fla::fla_recurrence_fwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_fwd_kernel");
-  return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, PAIR, LPR, 512>, "fla_recurrence_bwd_kernel")
-                  : go(fla::fla_recurrence_fwd_kernel<TX, TG, PAIR, LPR, 1024>, "fla_recurrence_fwd_kernel");
+    return backward ? go(fla::fla_recurrence_direct_bwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_direct_bwd_kernel")
+                    : go(fla::fla_recurrence_direct_fwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_direct_fwd_kernel");
+  return backward ? go(fla::fla_recurrence_direct_bwd_kernel<TX, TG, PAIR, LPR, 512>, "fla_recurrence_direct_bwd_kernel")
+                  : go(fla::fla_recurrence_direct_fwd_kernel<TX, TG, PAIR, LPR, 1024>, "fla_recurrence_direct_fwd_kernel");
 }
 
 template <typename TX, typename TG>
