@@ -54,7 +54,7 @@ struct RecurrenceParams {
 };
 
 constexpr int kShortThreads = 128;
-constexpr int kRecMaxCluster = 8;
+constexpr int kRecMaxCluster = 8;  // (what the exchange holds in registers)
 
 // Tokens a thread holds: a run. 16-bit rows and gates leave room for twice as many.
 template <typename TX, typename TG>
@@ -257,14 +257,22 @@ __global__ void __launch_bounds__(kShortThreads) fla_recurrence_short_bwd_kernel
 // ------------------------------------------------------------------------------------------------------------
 // Clusters of CTAs that walk a tile of 2 LPR channels together, a step of ranks * runs * T tokens at a time.
 
+// What the threads of a CTA, and the CTAs of a cluster, hand each other of a step.
+struct JoinSpace {
+  RunMap* run;      // [run of the CTA][lane]
+  float2* before;   // the same: a run's sum of gates, and then the state before it
+  float4* factor;   // [step parity][rank][lane]: hi and lo of the CTAs' maps
+  float2* b;        // the same
+  uint64_t* arrived;  // [step parity]: barriers
+};
 template <int LPR, int THREADS>
 struct RecurrenceShared {
-  RunMap run[THREADS];     // [run of the CTA][lane]
-  float2 before[THREADS];  // its sum of gates, and then the state before it
-  // What the CTAs of the cluster send each other: [step parity][rank][lane], and a barrier for each parity.
-  float4 factor[2][kRecMaxCluster][LPR];  // hi, lo
-  float2 b[2][kRecMaxCluster][LPR];
+  RunMap run[THREADS];
+  float2 before[THREADS];
+  float4 factor[2 * kRecMaxCluster * LPR];
+  float2 b[2 * kRecMaxCluster * LPR];
   uint64_t arrived[2];
+  __device__ __forceinline__ JoinSpace space() { return {run, before, factor, b, arrived}; }
 };
 struct Team {
   int lane, run, rank, ranks;
@@ -300,12 +308,13 @@ __device__ __forceinline__ bool maps_arrived(uint32_t barrier, uint32_t phase, u
 // their bytes at the receiver's barrier when they have arrived: unlike a barrier of the cluster, they need no fence, and
 // so do not wait for the rows that were written to memory before (5 us a step that way, 2.5 this way). A peer
 // writes to a slot again two steps later, for which it needs what this CTA sends when it has read the slot.
-template <int LPR, int THREADS>
-__device__ __forceinline__ bool trade_maps(RecurrenceShared<LPR, THREADS>& sh, int step, const RunMap& all, const Team& w,
+template <int LPR>
+__device__ __forceinline__ bool trade_maps(const JoinSpace& sh, int step, const RunMap& all, const Team& w,
                                            const RecurrenceParams& p) {
   const int parity = step & 1;
-  const uint32_t factor = shared_address(&sh.factor[parity][w.rank][w.lane]), b = shared_address(&sh.b[parity][w.rank][w.lane]);
-  const uint32_t barrier = shared_address(&sh.arrived[parity]);
+  const uint32_t factor = shared_address(sh.factor + (parity * kRecMaxCluster + w.rank) * LPR + w.lane);
+  const uint32_t b = shared_address(sh.b + (parity * kRecMaxCluster + w.rank) * LPR + w.lane);
+  const uint32_t barrier = shared_address(sh.arrived + parity);
   if (w.lane == 0)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(w.ranks * LPR * 24) : "memory");
   if (!(p.withhold && step == 0 && w.rank == 0)) {
@@ -323,56 +332,84 @@ __device__ __forceinline__ bool trade_maps(RecurrenceShared<LPR, THREADS>& sh, i
   return maps_arrived(barrier, (step >> 1) & 1, p.wait_limit_ns);
 }
 
-// Exchanges the maps of a step and returns the state before this thread's run. `carry`, which the first run's threads
-// hold, is the state before the step and becomes the one behind it. Runs and ranks count in the direction of the walk.
-// One warp joins them: all warps doing so for themselves issued a tenth of the kernel's instructions. `lost`: a wait has
-// run out; the state is NaN from there on, and nothing is sent or waited for any more.
+// Joins the maps of the runs of a step, in their order: the state before each run goes to `before`. `carry` is the state
+// before the step and becomes the one behind it. Runs and ranks count in the direction of the walk. One thread a pair of
+// channels does it (all warps doing so for themselves issued a tenth of the kernel's instructions). `lost`: a wait has run
+// out; the state is NaN from there on, and nothing is sent or waited for any more.
+template <int LPR, int RUNS>
+__device__ __forceinline__ void join(const JoinSpace& sh, int step, const Team& w, const RecurrenceParams& p, float2& carry, bool& lost) {
+  // (eight maps at a time in registers: loads between the steps of the chain cost 100 cycles a run)
+  constexpr int kSome = 8;
+  static_assert(RUNS % kSome == 0 && kRecMaxCluster == kSome, "");
+  RunMap m[kSome];
+  auto some = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < kSome; ++i) m[i] = sh.run[(from + i) * LPR + w.lane];
+  };
+  float2 c = carry;
+  if (w.ranks > 1) {
+    float2 sum = make_float2(0.f, 0.f), b = sum;
+#pragma unroll
+    for (int from = 0; from < RUNS; from += kSome) {
+      float2 sums[kSome];
+#pragma unroll
+      for (int i = 0; i < kSome; ++i) sums[i] = sh.before[(from + i) * LPR + w.lane];
+      some(from);
+#pragma unroll
+      for (int i = 0; i < kSome; ++i) {
+        sum = add2(sum, sums[i]);
+        b = apply_map(b, m[i]);
+      }
+    }
+    if (!lost && !trade_maps<LPR>(sh, step, run_map(sum, b), w, p)) {
+      lost = true;
+      if (p.status != nullptr) atomicOr(p.status, 1);
+    }
+#pragma unroll
+    for (int r = 0; r < kRecMaxCluster; ++r) {
+      const int at = ((step & 1) * kRecMaxCluster + (r < w.ranks ? r : 0)) * LPR + w.lane;
+      const float4 f = sh.factor[at];
+      m[r].hi = make_float2(f.x, f.y);
+      m[r].lo = make_float2(f.z, f.w);
+      m[r].b = sh.b[at];
+    }
+    float2 before = c;
+#pragma unroll
+    for (int r = 0; r < kRecMaxCluster; ++r)
+      if (r < w.ranks) {
+        if (r == w.rank) before = c;
+        c = apply_map(c, m[r]);
+      }
+    if (lost) c = before = make_float2(NAN, NAN);
+    carry = c;
+    c = before;
+  }
+#pragma unroll
+  for (int from = 0; from < RUNS; from += kSome) {
+    some(from);
+#pragma unroll
+    for (int i = 0; i < kSome; ++i) {
+      sh.before[(from + i) * LPR + w.lane] = c;
+      c = apply_map(c, m[i]);
+    }
+  }
+  if (w.ranks == 1) carry = c;
+}
+
+// The exchange of a step by the threads that work on it: the first run's join, the others wait for them.
 template <int LPR, int THREADS>
 __device__ __forceinline__ float2 exchange(RecurrenceShared<LPR, THREADS>& sh, int step, float2 sum, float2 b, const Team& w,
                                            const RecurrenceParams& p, float2& carry, bool& lost) {
-  constexpr int kRuns = THREADS / LPR;
   sh.run[w.run * LPR + w.lane] = run_map(sum, b);
   sh.before[w.run * LPR + w.lane] = sum;
   __syncthreads();
-  if (w.run == 0) {
-    float2 c = carry;
-    if (w.ranks > 1) {
-#pragma unroll
-      for (int r = 1; r < kRuns; ++r) {
-        sum = add2(sum, sh.before[r * LPR + w.lane]);
-        b = apply_map(b, sh.run[r * LPR + w.lane]);
-      }
-      if (!lost && !trade_maps<LPR, THREADS>(sh, step, run_map(sum, b), w, p)) {
-        lost = true;
-        if (p.status != nullptr) atomicOr(p.status, 1);
-      }
-      float2 before = c;
-      for (int r = 0; r < w.ranks; ++r) {
-        const float4 f = sh.factor[step & 1][r][w.lane];
-        RunMap m;
-        m.hi = make_float2(f.x, f.y);
-        m.lo = make_float2(f.z, f.w);
-        m.b = sh.b[step & 1][r][w.lane];
-        if (r == w.rank) before = c;
-        c = apply_map(c, m);
-      }
-      if (lost) c = before = make_float2(NAN, NAN);
-      carry = c;
-      c = before;
-    }
-#pragma unroll
-    for (int r = 0; r < kRuns; ++r) {
-      sh.before[r * LPR + w.lane] = c;
-      c = apply_map(c, sh.run[r * LPR + w.lane]);
-    }
-    if (w.ranks == 1) carry = c;
-  }
+  if (w.run == 0) join<LPR, THREADS / LPR>(sh.space(), step, w, p, carry, lost);
   __syncthreads();
   return sh.before[w.run * LPR + w.lane];
 }
 
-template <bool PAIR, int LPR, int THREADS>
-__device__ __forceinline__ void take_place(const RecurrenceParams& p, RecurrenceShared<LPR, THREADS>& sh, Team* team, Place* w) {
+template <bool PAIR, int LPR>
+__device__ __forceinline__ void take_place(const RecurrenceParams& p, uint64_t* arrived, Team* team, Place* w) {
   cg::cluster_group cluster = cg::this_cluster();
   team->lane = threadIdx.x % LPR;
   team->run = threadIdx.x / LPR;
@@ -381,7 +418,7 @@ __device__ __forceinline__ void take_place(const RecurrenceParams& p, Recurrence
   *w = place<PAIR, LPR>(p, blockIdx.x / team->ranks, team->lane);
   if (threadIdx.x == 0 && team->ranks > 1) {
     for (int i = 0; i < 2; ++i)
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&sh.arrived[i])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(arrived + i)) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 }
@@ -396,12 +433,6 @@ __device__ __forceinline__ void anew(R (&v)[T]) {
   for (int t = 0; t < T; ++t) anew(v[t]);
 }
 
-__device__ __forceinline__ void load_after(uint32_t& r, const char* q, float after) {
-  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(q), "f"(after));
-}
-__device__ __forceinline__ void load_after(float2& r, const char* q, float after) {
-  asm volatile("ld.global.nc.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "l"(q), "f"(after));
-}
 __device__ __forceinline__ void load_after(uint16_t& r, const char* q, float after) {
   asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(r) : "l"(q), "f"(after));
 }
@@ -411,7 +442,7 @@ __device__ __forceinline__ void load_after(float& r, const char* q, float after)
 
 // A thread's two columns of the rows of a step: the rows' base is the same for the CTA, offsets inside a step fit 32 bits
 // (checked on the host). Columns past the last read the first one's and are not written.
-template <typename T, bool PAIR>
+template <typename T>
 struct Rows {
   char* base;  // of the batch entry and head
   uint32_t at, gap, row;  // bytes
@@ -428,18 +459,13 @@ struct Rows {
   // `after`: the load is issued behind what this value comes from, whose operands' registers it can take.
   __device__ __forceinline__ typename PairOf<T>::Raw load(const char* step, uint32_t token, float after) const {
     const char* q = step + (at + token * row);
-    typename PairOf<T>::Raw r;
-    if (PAIR) {
-      load_after(r, q, after);
-      return r;
-    }
     typename PairOf<T>::Element a, b;
     load_after(a, q, after);
     load_after(b, q + gap, after);
     return join_pair(a, b);
   }
   __device__ __forceinline__ void store(char* step, uint32_t token, const Place& w, float2 v) const {
-    store_pair<T, PAIR>(reinterpret_cast<T*>(step + (at + token * row)), w.gap, w.ok0, w.ok1, v);
+    store_pair<T, false>(reinterpret_cast<T*>(step + (at + token * row)), w.gap, w.ok0, w.ok1, v);
   }
 };
 
@@ -471,20 +497,20 @@ struct InMemory {
   }
 };
 
-template <typename TX, typename TG, bool PAIR, int LPR, int THREADS>
+template <typename TX, typename TG, int LPR, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_direct_fwd_kernel(const RecurrenceParams p) {
   constexpr int T = kRunTokens<TX, TG>;
   __shared__ RecurrenceShared<LPR, THREADS> sh;
   Team team;
   Place w;
-  take_place<PAIR>(p, sh, &team, &w);
+  take_place<false, LPR>(p, sh.arrived, &team, &w);
   bool lost = false;
   const int first = (team.rank * (THREADS / LPR) + team.run) * T;  // of the step's tokens
-  Rows<TX, PAIR> xr(p.x, w, first), orow(p.o, w, first);
-  Rows<TG, PAIR> gr(p.g, w, first);
+  Rows<TX> xr(p.x, w, first), orow(p.o, w, first);
+  Rows<TG> gr(p.g, w, first);
   const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
   float2 carry = make_float2(0.f, 0.f);
-  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, false>(p.start + cell, w.gap, w.ok0, w.ok1);
 
   const int span = team.ranks * (THREADS / LPR) * T;  // tokens a step
   const int steps = (p.n - 1) / span + 1, runs_all = (p.n - 1) / T + 1;
@@ -518,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_direct
     }
     h = exchange(sh, step, sum, h, team, p, carry, lost);
     if (p.states != nullptr && t0 < p.n)
-      store_pair<float, PAIR>(p.states + state_of(p, w, t0 / T, runs_all), w.gap, w.ok0, w.ok1, h);
+      store_pair<float, false>(p.states + state_of(p, w, t0 / T, runs_all), w.gap, w.ok0, w.ok1, h);
     char* os = orow.step(p.o, static_cast<long long>(step) * span);
     anew(x);
     anew(g);
@@ -545,27 +571,27 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_direct
     }
   }
   if (p.end != nullptr && team.run == 0 && team.rank == 0)
-    store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
+    store_pair<float, false>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
   if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
 }
 
-template <typename TX, typename TG, bool PAIR, int LPR, int THREADS>
+template <typename TX, typename TG, int LPR, int THREADS>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_bwd_kernel(const RecurrenceParams p) {
   constexpr int T = kRunTokens<TX, TG>;
   __shared__ RecurrenceShared<LPR, THREADS> sh;
   Team team;
   Place w;
-  take_place<PAIR>(p, sh, &team, &w);
+  take_place<false, LPR>(p, sh.arrived, &team, &w);
   bool lost = false;
   const int span = team.ranks * (THREADS / LPR);                        // runs a step
   const int nth = span - 1 - (team.rank * (THREADS / LPR) + team.run);  // of the step's runs, in the order of the tokens
   const int first = nth * T;
-  Rows<TX, PAIR> xr(p.x, w, first), yr(p.o, w, first), dxr(p.dx, w, first);
-  Rows<TG, PAIR> gr(p.g, w, first), dgr(p.dg, w, first);
+  Rows<TX> xr(p.x, w, first), yr(p.o, w, first), dxr(p.dx, w, first);
+  Rows<TG> gr(p.g, w, first), dgr(p.dg, w, first);
   const bool has_dy = p.o.ptr != nullptr, want_dx = p.dx.ptr != nullptr, want_dg = p.dg.ptr != nullptr;
   const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
   float2 carry = make_float2(0.f, 0.f);
-  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, PAIR>(p.start + cell, w.gap, w.ok0, w.ok1);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, false>(p.start + cell, w.gap, w.ok0, w.ok1);
 
   const int runs_all = (p.n - 1) / T + 1;
   const int steps = (runs_all - 1) / span + 1;
@@ -587,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_
   auto load_state = [&](int step) {
     state = make_float2(0.f, 0.f);
     const int run = step * span + nth;
-    if (run < runs_all) state = load_pair<float, PAIR>(p.states + state_of(p, w, run, runs_all), w.gap, w.ok0, w.ok1);
+    if (run < runs_all) state = load_pair<float, false>(p.states + state_of(p, w, run, runs_all), w.gap, w.ok0, w.ok1);
   };
   load_state(steps - 1);
 #pragma unroll
@@ -667,55 +693,95 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_
     }
   }
   if (p.end != nullptr && team.run == 0 && team.rank == 0)
-    store_pair<float, PAIR>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
+    store_pair<float, false>(p.end + cell, w.gap, w.ok0, w.ok1, carry);
   if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// The same with rows that lie on 16-byte boundaries: a warp brings the rows of its runs of the next steps into a tile of its
-// own in shared memory, 16 bytes a lane and asynchronously, takes them into registers, and lets results leave the same
-// way. The loads of a step so are on their way through the whole step before, its exchange included, and there are a
-// quarter as many of them.
+// The same with rows that lie on 4-byte boundaries, or better on 16: a warp brings the rows of its runs of the next steps into
+// a tile of its own in shared memory, asynchronously, and lets results leave the same way. The loads of a step so are on
+// their way through the whole step before, its exchange included, and with 16 bytes a lane there are a quarter as many.
 
-// T-typed rows of the runs of a warp: TOK tokens each, 2 LPR columns.
-template <typename T, int LPR, int TOK>
+// T-typed rows of the runs of a warp: TOK tokens each, 2 LPR columns, copied in pieces of PIECE bytes: 16, or 4 where
+// rows are aligned to no more.
+template <typename T, int LPR, int TOK, int PIECE>
 struct WarpTile {
-  static constexpr int kRow = 2 * LPR * sizeof(T), kPieces = kRow / 16, kRows = TOK * (32 / LPR);
-  static constexpr int kBytes = kRows * kRow, kEach = kBytes / 512, kRowsEach = 32 / kPieces;
-  char* base;                // of the batch entry, head and tile of channels
-  uint32_t at, row, first;   // bytes; the lane's first row of the warp's
-  bool in;                   // its piece lies inside the row
+  static constexpr int kRow = 2 * LPR * sizeof(T), kPieces = kRow / PIECE, kRows = TOK * (32 / LPR);
+  static constexpr int kBytes = kRows * kRow, kEach = kBytes / (32 * PIECE);
+  static constexpr int kRowsEach = kPieces < 32 ? 32 / kPieces : 1, kParts = kPieces > 32 ? kPieces / 32 : 1;  // a row a turn, or parts of it
+  char* base;                     // of the batch entry, head and tile of channels
+  uint32_t at, row;               // bytes
+  int first, left_in_row;         // the lane's first row of the warp's; bytes of the row from its piece on
+  bool whole;                     // every piece lies inside the row
 
   __device__ __forceinline__ WarpTile(const RecurrenceTensor& t, const Place& w, int tile_column, int columns, int first_token) {
     base = static_cast<char*>(t.ptr) + (w.b * t.sb + w.h * t.sh + tile_column) * static_cast<long long>(sizeof(T));
     row = static_cast<uint32_t>(t.sn) * sizeof(T);
     const int lane = threadIdx.x % 32, piece = lane % kPieces;
     first = lane / kPieces;
-    at = (first_token + first) * row + piece * 16;
-    in = piece * 16 < columns * static_cast<int>(sizeof(T));
+    at = (first_token + first) * row + piece * PIECE;
+    left_in_row = columns * static_cast<int>(sizeof(T)) - piece * PIECE;
+    whole = columns >= 2 * LPR;
   }
   __device__ __forceinline__ char* step(const RecurrenceTensor& t, long long token) const {
     return base + token * t.sn * static_cast<long long>(sizeof(T));
   }
+  __device__ __forceinline__ bool inside(int k, int left) const {
+    return k % kParts * 32 * PIECE < left_in_row && first + k / kParts * kRowsEach < left;
+  }
+  __device__ __forceinline__ uint32_t offset(int k) const { return k / kParts * kRowsEach * row + k % kParts * 32 * PIECE; }
   // Rows past the last token (`left`: how many of the warp's rows there are) are zero, the identity.
   __device__ __forceinline__ void copy(uint32_t tile, const char* step, int left) const {
+    const char* from = step + at;
+    const uint32_t to = tile + threadIdx.x % 32 * PIECE;
+    const bool all = left >= kRows && whole;
+    if constexpr (PIECE == 16) {
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const bool ok = in && static_cast<int>(first) + k * kRowsEach < left;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + (k * 32 + threadIdx.x % 32) * 16),
-                   "l"(ok ? step + (at + k * kRowsEach * row) : base), "r"(ok ? 16 : 0)
-                   : "memory");
+      for (int k = 0; k < kEach; ++k) {
+        if (all) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * 512), "l"(from + offset(k)) : "memory");
+        } else {
+          const bool ok = inside(k, left);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * 512), "l"(ok ? from + offset(k) : base), "r"(ok ? 16 : 0)
+                       : "memory");
+        }
+      }
+    } else {
+      // (four times as many: addresses are advanced, and whole tiles make no choices, which were half of all instructions)
+      const uint32_t next = kRowsEach * row;
+      if (all) {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + k * 128), "l"(from + k % kParts * 128) : "memory");
+          if (k % kParts == kParts - 1) from += next;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          const bool ok = inside(k, left);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + k * 128), "l"(ok ? from + k % kParts * 128 : base), "r"(ok ? 4 : 0)
+                       : "memory");
+          if (k % kParts == kParts - 1) from += next;
+        }
+      }
     }
   }
   __device__ __forceinline__ void store(uint32_t tile, char* step, int left) const {
+    char* to = step + at;
+    const bool all = left >= kRows && whole;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      uint4 v;
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                   : "r"(tile + (k * 32 + threadIdx.x % 32) * 16)
-                   : "memory");
-      if (in && static_cast<int>(first) + k * kRowsEach < left) *reinterpret_cast<uint4*>(step + (at + k * kRowsEach * row)) = v;
+      const uint32_t from = tile + (k * 32 + threadIdx.x % 32) * PIECE;
+      if constexpr (PIECE == 16) {
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+        if (all || inside(k, left)) *reinterpret_cast<uint4*>(to + offset(k)) = v;
+      } else {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+        if (all || inside(k, left)) *reinterpret_cast<uint32_t*>(to + k % kParts * 128) = v;
+        if (k % kParts == kParts - 1) to += kRowsEach * row;
+      }
     }
   }
   // A token's two channels of a thread, whose run's rows begin at `run`.
@@ -742,108 +808,175 @@ __device__ __forceinline__ void copies_wait() {
   __syncwarp();
 }
 
-constexpr int kFwdStages = 2;
+// Forward, eight warps work on runs and a ninth joins them, a step apart: while it joins the runs of one step, the others sum those
+// of the next (first walk), and then finish the one before (second walk). With both on the same step (two barriers in a
+// row, each waiting for a chain of one or two thousand cycles) the warps stood still for two fifths of the time.
+// Three steps' tiles a warp: one that waits for its second walk, one in its first, one on its way. Results take the place
+// of what they come from, and the tile is free when they have left.
+constexpr int kTileThreads = 256, kTileSteps = 3;
+template <int LPR>
+constexpr int kJoinBytes = 2 * (kTileThreads * static_cast<int>(sizeof(RunMap) + sizeof(float2))) + 16;
+template <int LPR>
+constexpr int kTradeBytes = 2 * kRecMaxCluster * LPR * 24;
 template <typename TX, typename TG, int LPR>
-constexpr int kFwdWarpBytes = kFwdStages * (WarpTile<TX, LPR, kRunTokens<TX, TG>>::kBytes + WarpTile<TG, LPR, kRunTokens<TX, TG>>::kBytes) +
-                              WarpTile<TX, LPR, kRunTokens<TX, TG>>::kBytes;
+constexpr int kFwdTile = kRunTokens<TX, TG> * 64 * static_cast<int>(sizeof(TX) + sizeof(TG));
+// Backward, whose tiles are larger and whose walks need more registers, two CTAs an SM with one tile a warp (and room for the
+// results) each do better than one CTA a step apart: 4 x 32 heads, 8192 x 128 in bf16 235 against 336 us.
 template <typename TX, typename TG, int LPR>
-constexpr int kBwdWarpBytes = 3 * WarpTile<TX, LPR, kRunTokens<TX, TG>>::kBytes + 2 * WarpTile<TG, LPR, kRunTokens<TX, TG>>::kBytes;
+constexpr int kBwdTile = kRunTokens<TX, TG> * 64 * static_cast<int>(3 * sizeof(TX) + 2 * sizeof(TG));
 
-template <typename TX, typename TG, int LPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_fwd_kernel(const RecurrenceParams p) {
-  constexpr int T = kRunTokens<TX, TG>, kRuns = THREADS / LPR;
-  using TileX = WarpTile<TX, LPR, T>;
-  using TileG = WarpTile<TG, LPR, T>;
-  extern __shared__ uint4 tiles[];
-  __shared__ RecurrenceShared<LPR, THREADS> sh;
-  Team team;
-  Place w;
-  take_place<true>(p, sh, &team, &w);
-  bool lost = false;
-  const int column = w.c0 - 2 * team.lane;  // of the tile
-  const int first = (team.rank * kRuns + team.run / (32 / LPR) * (32 / LPR)) * T;  // of the warp's tokens, in the step
-  const int mine = team.run % (32 / LPR) * T;                                      // of the run's, among them
-  const TileX xt(p.x, w, column, p.c - column, first), ot(p.o, w, column, p.c - column, first);
-  const TileG gt(p.g, w, column, p.c - column, first);
-  const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kFwdWarpBytes<TX, TG, LPR>;
-  const uint32_t out = space + kFwdStages * (TileX::kBytes + TileG::kBytes);
-  const uint32_t x_run = mine * TileX::kRow + team.lane * 2 * sizeof(TX), g_run = mine * TileG::kRow + team.lane * 2 * sizeof(TG);
+// The joining warp's and the others' ends of the two hand-overs of a step.
+enum { kMapsReady = 1, kStatesReady = 3 };  // + step parity
+__device__ __forceinline__ void hand_over(int barrier) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "n"(kTileThreads + 32) : "memory");
+}
+__device__ __forceinline__ void take_over(int barrier) {
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kTileThreads + 32) : "memory");
+}
+
+// Shared memory: the warps' tiles, [parity] maps, [parity] sums and states, barriers, and in a cluster what is traded.
+template <int LPR>
+__device__ __forceinline__ JoinSpace join_space(char* after_tiles, int parity) {
+  JoinSpace j;
+  j.factor = reinterpret_cast<float4*>(after_tiles + kJoinBytes<LPR>);
+  j.b = reinterpret_cast<float2*>(j.factor + 2 * kRecMaxCluster * LPR);
+  j.run = reinterpret_cast<RunMap*>(after_tiles) + parity * kTileThreads;
+  j.before = reinterpret_cast<float2*>(after_tiles + 2 * kTileThreads * sizeof(RunMap)) + parity * kTileThreads;
+  j.arrived = reinterpret_cast<uint64_t*>(after_tiles + kJoinBytes<LPR> - 16);
+  return j;
+}
+template <int LPR, int PIECE>
+__device__ __forceinline__ void join_steps(const RecurrenceParams& p, char* after_tiles, Team team, const Place& w, int steps) {
+  const bool active = team.lane == static_cast<int>(threadIdx.x % 32);  // (LPR = 16: half of the warp)
   const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
   float2 carry = make_float2(0.f, 0.f);
-  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, true>(p.start + cell, 1, w.ok0, w.ok1);
+  bool lost = false;
+  if (p.start != nullptr) carry = load_pair<float, PIECE == 16>(p.start + cell, 1, w.ok0, w.ok1);
+  for (int step = 0; step < steps; ++step) {
+    take_over(kMapsReady + (step & 1));
+    if (active) join<LPR, kTileThreads / LPR>(join_space<LPR>(after_tiles, step & 1), step, team, p, carry, lost);
+    __syncwarp();
+    hand_over(kStatesReady + (step & 1));
+  }
+  if (active && p.end != nullptr && team.rank == 0) store_pair<float, PIECE == 16>(p.end + cell, 1, w.ok0, w.ok1, carry);
+}
 
+template <typename TX, typename TG, int LPR, int PIECE>
+__global__ void __launch_bounds__(kTileThreads + 32, 2) fla_recurrence_fwd_kernel(const RecurrenceParams p) {
+  constexpr int T = kRunTokens<TX, TG>, kRuns = kTileThreads / LPR, kWarpRuns = 32 / LPR;
+  using TileX = WarpTile<TX, LPR, T, PIECE>;
+  using TileG = WarpTile<TG, LPR, T, PIECE>;
+  constexpr int kTile = kFwdTile<TX, TG, LPR>;
+  extern __shared__ uint4 tiles[];
+  char* const after_tiles = reinterpret_cast<char*>(tiles) + kTileThreads / 32 * kTileSteps * kTile;
+  Team team;
+  Place w;
+  take_place<true, LPR>(p, join_space<LPR>(after_tiles, 0).arrived, &team, &w);
   const int span = team.ranks * kRuns * T;  // tokens a step
   const int steps = (p.n - 1) / span + 1, runs_all = (p.n - 1) / T + 1;
-  auto bring = [&](int step) {
-    const uint32_t slot = space + step % kFwdStages * (TileX::kBytes + TileG::kBytes);
-    const long long token = static_cast<long long>(step) * span;
-    const int left = step < steps ? p.n - step * span - first : 0;
-    xt.copy(slot, xt.step(p.x, token), left);
-    gt.copy(slot + TileX::kBytes, gt.step(p.g, token), left);
-    copies_end();
-  };
-#pragma unroll
-  for (int s = 0; s < kFwdStages; ++s) bring(s);
-  if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
-  for (int step = 0; step < steps; ++step) {
-    const uint32_t slot = space + step % kFwdStages * (TileX::kBytes + TileG::kBytes);
-    typename PairOf<TX>::Raw x[T];
-    typename PairOf<TG>::Raw g[T];
-    copies_wait<kFwdStages - 1>();
-    float2 sum = make_float2(0.f, 0.f), h = sum;
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      x[t] = TileX::get(slot + x_run, t);
-      g[t] = TileG::get(slot + TileX::kBytes + g_run, t);
-      const float2 gv = unpack_pair<TG>(g[t]);
-      sum = add2(sum, gv);
-      h = advance<TX, false>(gv, h, unpack_pair<TX>(x[t]));
-    }
-    __syncwarp();  // every lane has its rows: the tile is free
-    bring(step + kFwdStages);
-    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
-    if (drops) {
-      const InMemory<typename PairOf<TX>::Raw, T> xm(x);
-      const InMemory<typename PairOf<TG>::Raw, T> gm(g);
-      h = advance_from<TX, TG, T>(make_float2(0.f, 0.f), xm.v, gm.v, nullptr);
-    }
-    h = exchange(sh, step, sum, h, team, p, carry, lost);
-    const int t0 = step * span + first + mine;
-    if (p.states != nullptr && t0 < p.n)
-      store_pair<float, true>(p.states + state_of(p, w, t0 / T, runs_all), 1, w.ok0, w.ok1, h);
-    anew(x);
-    anew(g);
-    if (!drops) {
+  if (threadIdx.x >= kTileThreads) {
+    if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
+    join_steps<LPR, PIECE>(p, after_tiles, team, w, steps);
+  } else {
+    const int column = w.c0 - 2 * team.lane;                                    // of the tile
+    const int first = (team.rank * kRuns + team.run / kWarpRuns * kWarpRuns) * T;  // of the warp's tokens, in the step
+    const int mine = team.run % kWarpRuns * T;                                  // of the run's, among them
+    const TileX xt(p.x, w, column, p.c - column, first), ot(p.o, w, column, p.c - column, first);
+    const TileG gt(p.g, w, column, p.c - column, first);
+    const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kTileSteps * kTile;
+    const uint32_t x_run = mine * TileX::kRow + team.lane * 2 * sizeof(TX);
+    const uint32_t g_run = TileX::kBytes + mine * TileG::kRow + team.lane * 2 * sizeof(TG);
+    const int cell = team.run * LPR + team.lane;
+    auto bring = [&](int step, uint32_t tile) {
+      const long long token = static_cast<long long>(step) * span;
+      const int left = step < steps ? p.n - step * span - first : 0;
+      xt.copy(tile, xt.step(p.x, token), left);
+      gt.copy(tile + TileX::kBytes, gt.step(p.g, token), left);
+      copies_end();
+    };
+    // The first walk: the run's sum from zero, and of its gates. True where one of them is minus infinity.
+    auto sum_up = [&](int step, uint32_t tile) {
+      float2 sum = make_float2(0.f, 0.f), h = sum;
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
-        TileX::put(out + x_run, t, h);
+        const float2 gv = unpack_pair<TG>(TileG::get(tile + g_run, t));
+        sum = add2(sum, gv);
+        h = fma2(decay<TX>(gv), h, unpack_pair<TX>(TileX::get(tile + x_run, t)));
       }
-    } else {
+      const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+      if (drops) {
+        h = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int t = 0; t < T; ++t)
+          h = advance<TX, true>(unpack_pair<TG>(TileG::get(tile + g_run, t)), h, unpack_pair<TX>(TileX::get(tile + x_run, t)));
+      }
+      const JoinSpace j = join_space<LPR>(after_tiles, step & 1);
+      j.run[cell] = run_map(sum, h);
+      j.before[cell] = sum;
+      hand_over(kMapsReady + (step & 1));
+      return drops;
+    };
+    bring(0, space);
+    bring(1, space + kTile);
+    bring(2, space + 2 * kTile);
+    if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
+    uint32_t tile = space, next = space + kTile, last = space + 2 * kTile;
+    copies_wait<2>();
+    bool drops = sum_up(0, tile);
+    for (int step = 0; step < steps; ++step) {
+      bool next_drops = false;
+      copies_wait<1>();
+      if (step + 1 < steps) next_drops = sum_up(step + 1, next);
+      take_over(kStatesReady + (step & 1));
+      float2 h = join_space<LPR>(after_tiles, step & 1).before[cell];
+      const int t0 = step * span + first + mine;
+      if (p.states != nullptr && t0 < p.n)
+        store_pair<float, PIECE == 16>(p.states + state_of(p, w, t0 / T, runs_all), 1, w.ok0, w.ok1, h);
+      if (!drops) {
+        // (all rows first: each load behind the store of the token before made the walk twice as long)
+        typename PairOf<TX>::Raw x[T];
+        float2 a[T];
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        h = advance<TX, true>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
-        TileX::put(out + x_run, t, h);
+        for (int t = 0; t < T; ++t) {
+          x[t] = TileX::get(tile + x_run, t);
+          a[t] = decay<TX>(unpack_pair<TG>(TileG::get(tile + g_run, t)));
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          h = fma2(a[t], h, unpack_pair<TX>(x[t]));
+          TileX::put(tile + x_run, t, h);
+        }
+      } else {
+#pragma unroll 1
+        for (int t = 0; t < T; ++t) {
+          h = advance<TX, true>(unpack_pair<TG>(TileG::get(tile + g_run, t)), h, unpack_pair<TX>(TileX::get(tile + x_run, t)));
+          TileX::put(tile + x_run, t, h);
+        }
       }
+      __syncwarp();
+      ot.store(tile, ot.step(p.o, static_cast<long long>(step) * span), p.n - step * span - first);
+      __syncwarp();
+      bring(step + kTileSteps, tile);
+      const uint32_t free = tile;
+      tile = next;
+      next = last;
+      last = free;
+      drops = next_drops;
     }
-    __syncwarp();
-    ot.store(out, ot.step(p.o, static_cast<long long>(step) * span), p.n - step * span - first);
-    __syncwarp();
   }
-  if (p.end != nullptr && team.run == 0 && team.rank == 0) store_pair<float, true>(p.end + cell, 1, w.ok0, w.ok1, carry);
   if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
 }
 
-template <typename TX, typename TG, int LPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_kernel(const RecurrenceParams p) {
-  constexpr int T = kRunTokens<TX, TG>, kRuns = THREADS / LPR, kWarpRuns = 32 / LPR;
-  using TileX = WarpTile<TX, LPR, T>;
-  using TileG = WarpTile<TG, LPR, T>;
+template <typename TX, typename TG, int LPR, int PIECE>
+__global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(const RecurrenceParams p) {
+  constexpr int T = kRunTokens<TX, TG>, kRuns = kTileThreads / LPR, kWarpRuns = 32 / LPR;
+  using TileX = WarpTile<TX, LPR, T, PIECE>;
+  using TileG = WarpTile<TG, LPR, T, PIECE>;
   extern __shared__ uint4 tiles[];
-  __shared__ RecurrenceShared<LPR, THREADS> sh;
+  __shared__ RecurrenceShared<LPR, kTileThreads> sh;
   Team team;
   Place w;
-  take_place<true>(p, sh, &team, &w);
+  take_place<true, LPR>(p, sh.arrived, &team, &w);
   bool lost = false;
   const int column = w.c0 - 2 * team.lane;
   const int span = team.ranks * kRuns;                        // runs a step
@@ -852,12 +985,12 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_ker
   const TileX xt(p.x, w, column, p.c - column, first), yt(p.o, w, column, p.o.ptr != nullptr ? p.c - column : 0, first);
   const TileX dxt(p.dx, w, column, p.dx.ptr != nullptr ? p.c - column : 0, first);
   const TileG gt(p.g, w, column, p.c - column, first), dgt(p.dg, w, column, p.dg.ptr != nullptr ? p.c - column : 0, first);
-  const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kBwdWarpBytes<TX, TG, LPR>;
+  const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kBwdTile<TX, TG, LPR>;
   const uint32_t y_at = space + TileX::kBytes, dx_at = space + 2 * TileX::kBytes, g_at = space + 3 * TileX::kBytes, dg_at = g_at + TileG::kBytes;
   const uint32_t x_run = mine * TileX::kRow + team.lane * 2 * sizeof(TX), g_run = mine * TileG::kRow + team.lane * 2 * sizeof(TG);
   const long long cell = static_cast<long long>(w.b * p.heads + w.h) * p.c + w.c0;
   float2 carry = make_float2(0.f, 0.f);
-  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, true>(p.start + cell, 1, w.ok0, w.ok1);
+  if (team.run == 0 && p.start != nullptr) carry = load_pair<float, PIECE == 16>(p.start + cell, 1, w.ok0, w.ok1);
 
   const int runs_all = (p.n - 1) / T + 1;
   const int steps = (runs_all - 1) / span + 1;
@@ -873,13 +1006,14 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_ker
     copies_end();
     state = make_float2(0.f, 0.f);
     const int run = step * span + nth;
-    if (step >= 0 && run < runs_all) state = load_pair<float, true>(p.states + state_of(p, w, run, runs_all), 1, w.ok0, w.ok1);
+    if (step >= 0 && run < runs_all)
+      state = load_pair<float, PIECE == 16>(p.states + state_of(p, w, run, runs_all), 1, w.ok0, w.ok1);
   };
   bring(steps - 1);
   if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
   // The walk starts at the end; the runs behind the last token are the identity.
   for (int step = steps - 1; step >= 0; --step) {
-    typename PairOf<TX>::Raw x[T], y[T];
+    typename PairOf<TX>::Raw y[T];
     typename PairOf<TG>::Raw g[T];
     copies_wait<0>();
     float2 sum = make_float2(0.f, 0.f), r = sum, h = state;
@@ -894,9 +1028,10 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_ker
     const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
     float2 before[T];  // the state before each token
     anew(g);
+    if (drops) {  // (out of line and from memory: in line the second copy of the loops cost 50 registers)
+      typename PairOf<TX>::Raw x[T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) x[t] = TileX::get(space + x_run, t);
-    if (drops) {
+      for (int t = 0; t < T; ++t) x[t] = TileX::get(space + x_run, t);
       const InMemory<typename PairOf<TX>::Raw, T> xm(x), ym(y);
       const InMemory<typename PairOf<TG>::Raw, T> gm(g);
       float2 bm[T];
@@ -908,7 +1043,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_ker
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         before[t] = h;
-        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(x[t]));
+        h = advance<TX, false>(unpack_pair<TG>(g[t]), h, unpack_pair<TX>(TileX::get(space + x_run, t)));
       }
     }
     __syncwarp();  // every lane has its rows: the tiles are free
@@ -943,7 +1078,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_bwd_ker
     dgt.store(dg_at, dgt.step(p.dg, token), left);
     __syncwarp();
   }
-  if (p.end != nullptr && team.run == 0 && team.rank == 0) store_pair<float, true>(p.end + cell, 1, w.ok0, w.ok1, carry);
+  if (p.end != nullptr && team.run == 0 && team.rank == 0) store_pair<float, PIECE == 16>(p.end + cell, 1, w.ok0, w.ok1, carry);
   if (team.ranks > 1) cg::this_cluster().sync();  // (nobody leaves while a peer that gave up early may still be written to)
 }
 
@@ -962,7 +1097,8 @@ int element_bytes(int dtype) { return dtype == FLA_DTYPE_F32 ? 4 : 2; }
 // other in every tensor are one row: narrow heads then fill a warp.
 struct Plan {
   RecurrenceParams p;
-  bool pair, wide;  // rows lie on boundaries of two elements, of 16 bytes
+  bool pair;        // two neighbouring columns can be read at once in every tensor
+  int piece;        // bytes that rows can be copied in: 16, 4, or 0
   int lpr;
   int batch;
   long long farthest;  // bytes from one token to the next, of the tensor where they are most
@@ -1021,39 +1157,48 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
                 return reinterpret_cast<uintptr_t>(t.ptr) % (2 * size) == 0 && (p.n == 1 || t.sn % 2 == 0) &&
                        (p.heads == 1 || t.sh % 2 == 0) && (plan.batch == 1 || t.sb % 2 == 0);
               });
-  plan.wide = plan.pair && p.c * sizes[0] % 16 == 0 && p.c * sizes[1] % 16 == 0 && every([&](const RecurrenceTensor& t, int size) {
-                return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && (p.n == 1 || t.sn * size % 16 == 0) &&
-                       (p.heads == 1 || t.sh * size % 16 == 0) && (plan.batch == 1 || t.sb * size % 16 == 0);
-              });
+  auto rows_on = [&](int bytes) {
+    return p.c * sizes[0] % bytes == 0 && p.c * sizes[1] % bytes == 0 && every([&](const RecurrenceTensor& t, int size) {
+             return reinterpret_cast<uintptr_t>(t.ptr) % bytes == 0 && (p.n == 1 || t.sn * size % bytes == 0) &&
+                    (p.heads == 1 || t.sh * size % bytes == 0) && (plan.batch == 1 || t.sb * size % bytes == 0);
+           });
+  };
+  plan.piece = plan.pair && rows_on(16) ? 16 : rows_on(4) ? 4 : 0;
   plan.farthest = 1;
   every([&](const RecurrenceTensor& t, int size) {
     plan.farthest = std::max(plan.farthest, t.sn * size);
     return true;
   });
-  plan.lpr = p.c <= 32 ? 16 : 32;
+  // Tiles of 64 columns, or of 32 where that leaves fewer lanes without one.
+  plan.lpr = (p.c + 31) / 32 * 32 * 10 < (p.c + 63) / 64 * 64 * 9 ? 16 : 32;
   p.tiles = (p.c + 2 * plan.lpr - 1) / (2 * plan.lpr);
   p.tiles_all = static_cast<long long>(p.tiles) * p.heads * plan.batch;
   return plan;
 }
 
-// CTAs of a cluster and threads of a CTA. A tile of channels is walked by one cluster from end to end; more CTAs, and
-// larger ones, walk it in fewer steps.
+// CTAs of a cluster and threads of a CTA (that work on runs). A tile of channels is walked by one cluster from end to end;
+// more CTAs, and larger ones, walk it in fewer steps, of which each takes longer.
 struct Shape {
   int threads, ranks;
 };
-Shape shape_of(const Plan& plan, int run_tokens, int most_threads, int sm_count) {
+Shape shape_of(const Plan& plan, int run_tokens, bool backward, int sm_count) {
   const long long runs = (plan.p.n - 1) / run_tokens + 1;
   Shape s = {256, 1};
   auto step = [&] { return static_cast<long long>(s.ranks) * s.threads / plan.lpr; };
+  if (plan.piece) {  // one CTA an SM, backward two
+    const int most = backward ? 2 * sm_count : sm_count;
+    while (s.ranks < fla::kRecMaxCluster && plan.p.tiles_all * s.ranks * 2 <= most && step() < runs) s.ranks *= 2;
+    return s;
+  }
   while (s.ranks < fla::kRecMaxCluster && plan.p.tiles_all * s.ranks < 2 * sm_count && step() < runs) s.ranks *= 2;
-  if (plan.p.tiles_all * s.ranks <= sm_count && step() < runs) s.threads = most_threads;
+  if (plan.p.tiles_all * s.ranks <= sm_count && step() < runs) s.threads = backward ? 512 : 1024;
   return s;
 }
 
-template <typename TX, typename TG, bool PAIR, int LPR>
+template <typename TX, typename TG, int LPR>
 int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
   constexpr int T = fla::kRunTokens<TX, TG>;
-  Shape shape = shape_of(plan, T, backward || plan.wide ? 512 : 1024, sm_count);
+  Shape shape = shape_of(plan, T, backward, sm_count);
   const bool alone = plan.p.n <= kShortTokens || plan.farthest > 0x7fffffffLL / (shape.ranks * (shape.threads / LPR) * T);
   long long blocks = plan.p.tiles_all * shape.ranks;
   if (alone) {
@@ -1078,32 +1223,36 @@ int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
     return fla::launched(cudaLaunchKernelEx(&cfg, kernel, plan.p), name);
   };
   if (alone)
-    return backward ? go(fla::fla_recurrence_short_bwd_kernel<TX, TG, PAIR, LPR>, "fla_recurrence_short_bwd_kernel")
-                    : go(fla::fla_recurrence_short_fwd_kernel<TX, TG, PAIR, LPR>, "fla_recurrence_short_fwd_kernel");
-  if constexpr (PAIR) {
-    if (plan.wide) {
-      cfg.dynamicSmemBytes = shape.threads / 32 * (backward ? fla::kBwdWarpBytes<TX, TG, LPR> : fla::kFwdWarpBytes<TX, TG, LPR>);
-      if (shape.threads == 256)
-        return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 256>, "fla_recurrence_bwd_kernel")
-                        : go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 256>, "fla_recurrence_fwd_kernel");
-      return backward ? go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 512>, "fla_recurrence_bwd_kernel")
-                      : go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 512>, "fla_recurrence_fwd_kernel");
+    return plan.pair ? (backward ? go(fla::fla_recurrence_short_bwd_kernel<TX, TG, true, LPR>, "fla_recurrence_short_bwd_kernel")
+                                 : go(fla::fla_recurrence_short_fwd_kernel<TX, TG, true, LPR>, "fla_recurrence_short_fwd_kernel"))
+                     : (backward ? go(fla::fla_recurrence_short_bwd_kernel<TX, TG, false, LPR>, "fla_recurrence_short_bwd_kernel")
+                                 : go(fla::fla_recurrence_short_fwd_kernel<TX, TG, false, LPR>, "fla_recurrence_short_fwd_kernel"));
+  if (plan.piece) {
+    if (backward) {
+      cfg.dynamicSmemBytes = fla::kTileThreads / 32 * fla::kBwdTile<TX, TG, LPR>;
+      return plan.piece == 16 ? go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 16>, "fla_recurrence_bwd_kernel")
+                              : go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 4>, "fla_recurrence_bwd_kernel");
     }
+    cfg.blockDim = dim3(fla::kTileThreads + 32);
+    cfg.dynamicSmemBytes = fla::kTileThreads / 32 * fla::kTileSteps * fla::kFwdTile<TX, TG, LPR> + fla::kJoinBytes<LPR> +
+                           (shape.ranks > 1 ? fla::kTradeBytes<LPR> : 0);
+    return plan.piece == 16 ? go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 16>, "fla_recurrence_fwd_kernel")
+                            : go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 4>, "fla_recurrence_fwd_kernel");
   }
-  if (shape.threads == 256)
-    return backward ? go(fla::fla_recurrence_direct_bwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_direct_bwd_kernel")
-                    : go(fla::fla_recurrence_direct_fwd_kernel<TX, TG, PAIR, LPR, 256>, "fla_recurrence_direct_fwd_kernel");
-  return backward ? go(fla::fla_recurrence_direct_bwd_kernel<TX, TG, PAIR, LPR, 512>, "fla_recurrence_direct_bwd_kernel")
-                  : go(fla::fla_recurrence_direct_fwd_kernel<TX, TG, PAIR, LPR, 1024>, "fla_recurrence_direct_fwd_kernel");
+  if constexpr (sizeof(TX) == 4) {
+    return FLA_ERR_UNSUPPORTED;  // (fp32 rows always lie on 4 bytes)
+  } else {
+    if (shape.threads == 256)
+      return backward ? go(fla::fla_recurrence_direct_bwd_kernel<TX, TG, LPR, 256>, "fla_recurrence_direct_bwd_kernel")
+                      : go(fla::fla_recurrence_direct_fwd_kernel<TX, TG, LPR, 256>, "fla_recurrence_direct_fwd_kernel");
+    return backward ? go(fla::fla_recurrence_direct_bwd_kernel<TX, TG, LPR, 512>, "fla_recurrence_direct_bwd_kernel")
+                    : go(fla::fla_recurrence_direct_fwd_kernel<TX, TG, LPR, 1024>, "fla_recurrence_direct_fwd_kernel");
+  }
 }
 
 template <typename TX, typename TG>
 int launch_types(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
-  if (plan.pair)
-    return plan.lpr == 16 ? launch<TX, TG, true, 16>(plan, backward, sm_count, stream)
-                          : launch<TX, TG, true, 32>(plan, backward, sm_count, stream);
-  return plan.lpr == 16 ? launch<TX, TG, false, 16>(plan, backward, sm_count, stream)
-                        : launch<TX, TG, false, 32>(plan, backward, sm_count, stream);
+  return plan.lpr == 16 ? launch<TX, TG, 16>(plan, backward, sm_count, stream) : launch<TX, TG, 32>(plan, backward, sm_count, stream);
 }
 
 bool known_type(int t) { return t == FLA_DTYPE_BF16 || t == FLA_DTYPE_F16 || t == FLA_DTYPE_F32; }
