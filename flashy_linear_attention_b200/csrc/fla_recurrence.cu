@@ -1111,7 +1111,7 @@ void add_tensor(const FlaTensor& t, RecurrenceTensor* out) {
   out->sn = t.stride_n;
 }
 
-Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
+Plan make_plan(const FlaRecurrenceArgs* a, bool backward, int sm_count) {
   Plan plan = {};
   RecurrenceParams& p = plan.p;
   add_tensor(a->x, &p.x);
@@ -1169,8 +1169,12 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward) {
     plan.farthest = std::max(plan.farthest, t.sn * size);
     return true;
   });
-  // Tiles of 64 columns, or of 32 where that leaves fewer lanes without one.
-  plan.lpr = (p.c + 31) / 32 * 32 * 10 < (p.c + 63) / 64 * 64 * 9 ? 16 : 32;
+  // Tiles of 64 columns; of 32 where that leaves fewer lanes without one, and for few channels, whose clusters of eight would
+  // leave places on the SMs empty. Microseconds forward + backward with tiles of 64 and 32: 8 x 128 channels, 65536 tokens, bf16
+  // 215 + 306 / 128 + 214, fp32 403 + 531 / 204 + 303; 4 x 256 channels, 8192 tokens 38 + 44 / 23 + 34; but 32 x 128 channels,
+  // 2048 tokens 19 + 27 / 19 + 32, and 128 x 64 channels, 4096 tokens 48 + 82 / 52 + 89.
+  const long long tiles64 = (p.c + 63LL) / 64 * p.heads * plan.batch;
+  plan.lpr = (p.c + 31) / 32 * 32 * 10 < (p.c + 63) / 64 * 64 * 9 || tiles64 * fla::kRecMaxCluster <= 2 * sm_count ? 16 : 32;
   p.tiles = (p.c + 2 * plan.lpr - 1) / (2 * plan.lpr);
   p.tiles_all = static_cast<long long>(p.tiles) * p.heads * plan.batch;
   return plan;
@@ -1277,7 +1281,7 @@ int run(const FlaRecurrenceArgs* a, bool backward) {
   fla::g_last_launches = 0;
   int sm_count = 0;
   if (const int rc = fla::block_device(&sm_count)) return rc;
-  const Plan plan = make_plan(a, backward);
+  const Plan plan = make_plan(a, backward, sm_count);
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   const bool wide_gates = a->g_dtype == FLA_DTYPE_F32;
   if (a->dtype == FLA_DTYPE_F32) return launch_types<float, float>(plan, backward, sm_count, stream);
