@@ -11,11 +11,14 @@
 // drive other streams or GPUs, have to go on meanwhile.
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
 #include <array>
+#include <memory>
 #include <optional>
 #include <string>
 #include <vector>
@@ -588,6 +591,119 @@ std::optional<std::array<OptTensor, 3>> layer_norm_backward(const Tensor& dy, co
   return out;
 }
 
+// The Functions around these calls as native autograd nodes: a backward in Python has to be handed the interpreter lock by the
+// thread that waits for it, and a training step of a small layer took 90 us that way, of which 20 are these calls. The first
+// value of a result is empty where the call is not covered: the caller then takes the Python Functions of the same names.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients are not differentiable themselves; the error comes when somebody tries.
+variable_list once_differentiable(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    const auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", 1);
+    Tensor leaf = g.detach();
+    leaf.set_requires_grad(true);
+    g = error->apply({leaf})[0];
+  }
+  return grads;
+}
+bool wants_gradient(const Tensor& x, std::initializer_list<const OptTensor*> others) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const OptTensor* t : others)
+    if (t->has_value() && (*t)->requires_grad()) return true;
+  return x.requires_grad();
+}
+Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+OptTensor or_null(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+struct RecurrenceNode : torch::autograd::Function<RecurrenceNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const OptTensor& s_init, bool keep,
+                               int64_t debug_flags, int64_t status) {
+    const auto r = recurrence_forward(x, g, s_init, keep, static_cast<unsigned>(debug_flags), static_cast<uintptr_t>(status));
+    if (!r.has_value()) throw std::runtime_error("flashlinear: the recurrence's arguments changed between two checks");
+    if (keep) {
+      ctx->save_for_backward({x, g, or_none(r->states)});
+      ctx->saved_data["flags"] = debug_flags;
+      ctx->saved_data["status"] = status;
+      ctx->saved_data["wants"] = static_cast<int64_t>(x.requires_grad()) | static_cast<int64_t>(g.requires_grad()) << 1 |
+                                 static_cast<int64_t>(s_init.has_value() && s_init->requires_grad()) << 2;
+    }
+    ctx->set_materialize_grads(false);
+    return {r->out, r->s_final};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(6);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t wants = ctx->saved_data["wants"].toInt();
+    {
+      const at::AutoGradMode off(false);
+      const Tensor ds = grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : Tensor();
+      const auto r = recurrence_backward(or_null(grads[0]), saved[0], saved[1], saved[2], or_null(ds), wants & 1, wants & 2, wants & 4,
+                                         static_cast<unsigned>(ctx->saved_data["flags"].toInt()),
+                                         static_cast<uintptr_t>(ctx->saved_data["status"].toInt()));
+      if (!r.has_value()) throw std::runtime_error("flashlinear: the gradients of the recurrence's outputs do not fit them");
+      for (int i = 0; i < 3; ++i) out[i] = or_none((*r)[i]);
+    }
+    return once_differentiable(std::move(out));
+  }
+};
+
+// LayerNorm without, AddLayerNorm with a residual.
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& w, const OptTensor& b,
+                               double eps, bool keep) {
+    const auto r = layer_norm_forward(x, w, b, eps, residual, keep);
+    if (!r.has_value()) throw std::runtime_error("flashlinear: the layer norm's arguments changed between two checks");
+    if (keep) {
+      ctx->save_for_backward({residual.has_value() ? *r->sum : x, or_none(w), or_none(b), or_none(r->stats)});
+      ctx->saved_data["wants"] = static_cast<int64_t>(x.requires_grad() || (residual.has_value() && residual->requires_grad())) |
+                                 static_cast<int64_t>(w.has_value() && w->requires_grad()) << 1 |
+                                 static_cast<int64_t>(b.has_value() && b->requires_grad()) << 2;
+      ctx->saved_data["residual"] = residual.has_value();
+    }
+    ctx->set_materialize_grads(false);
+    if (residual.has_value()) return {r->out, *r->sum};
+    return {r->out};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(6);
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const Tensor ds = residual ? grads[1] : Tensor();
+    if (!grads[0].defined()) {  // the sum alone was used
+      out[0] = out[1] = ds;
+      return out;
+    }
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t wants = ctx->saved_data["wants"].toInt();
+    {
+      const at::AutoGradMode off(false);
+      auto rows = [&](const Tensor& t) { return !t.defined() || norm_rows(t, saved[0]) ? t : t.contiguous(); };
+      const auto r = layer_norm_backward(rows(grads[0]), saved[0], or_null(saved[1]), or_null(saved[2]), saved[3], or_null(rows(ds)),
+                                         wants & 1, wants & 2, wants & 4);
+      if (!r.has_value()) throw std::runtime_error("flashlinear: the gradients of the layer norm's outputs do not fit them");
+      out[0] = or_none((*r)[0]);
+      if (residual) out[1] = out[0];
+      out[2] = or_none((*r)[1]);
+      out[3] = or_none((*r)[2]);
+    }
+    return once_differentiable(std::move(out));
+  }
+};
+
+variable_list recurrence_apply(const Tensor& x, const Tensor& g, const OptTensor& s_init, unsigned debug_flags, uintptr_t status) {
+  if (!recurrence_covered(x, g) || !channel_state(s_init, x)) return {};
+  return RecurrenceNode::apply(x, g, s_init, g.requires_grad() && at::GradMode::is_enabled() ? true : wants_gradient(x, {&s_init}),
+                               static_cast<int64_t>(debug_flags), static_cast<int64_t>(status));
+}
+variable_list layer_norm_apply(const Tensor& x, const OptTensor& residual, const OptTensor& w, const OptTensor& b, double eps) {
+  if (!norm_covered(x, w, b) || (residual.has_value() && !norm_rows(*residual, x)) || !(eps >= 0)) return {};
+  return LayerNormNode::apply(x, residual, w, b, eps, wants_gradient(x, {&residual, &w, &b}));
+}
+
 // What is saved beside the repacked copy of an input that is not kept itself: an empty tensor that shares
 // its version count, for autograd to see that it was changed in place. (An inference tensor has none;
 // it is returned itself, and autograd refuses it as it always does.)
@@ -615,6 +731,8 @@ PYBIND11_MODULE(_hostcalls, m) {
     return py::make_tuple(r->out, r->s_final, r->seg_states, views);
   });
   m.def("version_of", &version_of);
+  m.def("recurrence_apply", &recurrence_apply, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm_apply", &layer_norm_apply, py::call_guard<py::gil_scoped_release>());
   m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, const OptTensor& residual,
                                  bool keep_stats) -> py::object {
     std::optional<Norm> r;

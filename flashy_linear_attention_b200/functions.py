@@ -9,13 +9,14 @@ the reference's ``custom_fwd(cast_inputs=torch.bfloat16)`` does.
 from __future__ import annotations
 
 import functools
+import os
 from typing import Any, Tuple
 
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import layer_norm, ops, recurrence
+from . import _lib, layer_norm, ops, recurrence
 
 
 def _autocast_to_bf16(forward):
@@ -242,6 +243,14 @@ class TaylorLinearAttention(Function):
         return ops.taylor_backward_in_memory(grad_output, xq, xk, v, *features)
 
 
+def _native_node(x):
+    """The native host path, for Functions that have a node there. Not with FLA_DEBUG=1, where the status is read after every
+    call, the backward's included."""
+    if not x.is_cuda or os.environ.get("FLA_DEBUG", "0") == "1":
+        return None
+    return _lib.host()
+
+
 class GatedLinearRecurrence(Function):
     """Gated linear recurrence, a state of its own for every channel:
     ``h_t = exp(log_decay_t) h_{t-1} + x_t``, ``out_t = h_t``.
@@ -260,12 +269,19 @@ class GatedLinearRecurrence(Function):
     The reference has no counterpart.
     """
 
-    @staticmethod
-    def forward(ctx: Any, x, log_decay, s_init=None):
+    @classmethod
+    def apply(cls, x, log_decay, s_init=None):
         if torch.is_autocast_enabled("cuda"):
             x = x.to(torch.bfloat16)
             if log_decay.dtype != torch.float32:
                 log_decay = log_decay.to(torch.bfloat16)
+        # (a native autograd node, which the forward and backward below stand in for where it does not cover the call)
+        native = _native_node(x)
+        outs = () if native is None else native.recurrence_apply(x, log_decay, s_init, ops._debug_flags, ops._status_ptr(x))
+        return tuple(outs) or super().apply(x, log_decay, s_init)
+
+    @staticmethod
+    def forward(ctx: Any, x, log_decay, s_init=None):
         out, s_final, states = recurrence.recurrence_fwd(x, log_decay, s_init, any(ctx.needs_input_grad[:3]))
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, log_decay, states)
@@ -293,6 +309,12 @@ class LayerNorm(Function):
     The reference has no counterpart.
     """
 
+    @classmethod
+    def apply(cls, x, weight=None, bias=None, eps: float = 1e-5):
+        native = _native_node(x)
+        outs = () if native is None else native.layer_norm_apply(x, None, weight, bias, eps)
+        return outs[0] if outs else super().apply(x, weight, bias, eps)
+
     @staticmethod
     def forward(ctx: Any, x, weight=None, bias=None, eps: float = 1e-5):
         out, _, stats = layer_norm.layer_norm_fwd(x, weight, bias, eps, None, any(ctx.needs_input_grad[:3]))
@@ -315,6 +337,12 @@ class AddLayerNorm(Function):
     ``sum`` is the residual of the next block, and its gradient joins that of ``out`` in one pass backward: x and the
     residual get the same gradient. The reference has no counterpart.
     """
+
+    @classmethod
+    def apply(cls, x, residual, weight=None, bias=None, eps: float = 1e-5):
+        native = _native_node(x)
+        outs = () if native is None or residual is None else native.layer_norm_apply(x, residual, weight, bias, eps)
+        return tuple(outs) or super().apply(x, residual, weight, bias, eps)
 
     @staticmethod
     def forward(ctx: Any, x, residual, weight=None, bias=None, eps: float = 1e-5):
