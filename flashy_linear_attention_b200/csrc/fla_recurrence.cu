@@ -1185,12 +1185,14 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward, int sm_count) {
 struct Shape {
   int threads, ranks;
 };
-Shape shape_of(const Plan& plan, int run_tokens, bool backward, int sm_count) {
+Shape shape_of(const Plan& plan, int run_tokens, bool backward, bool two_resident, int sm_count) {
   const long long runs = (plan.p.n - 1) / run_tokens + 1;
   Shape s = {256, 1};
   auto step = [&] { return static_cast<long long>(s.ranks) * s.threads / plan.lpr; };
-  if (plan.piece) {  // one CTA an SM, backward two
-    const int most = backward ? 2 * sm_count : sm_count;
+  if (plan.piece) {
+    // Backward two CTAs an SM. Forward two where their tiles are small enough (16-bit rows with fp32 gates), else one in a
+    // cluster: its CTAs all have to be there at once.
+    const int most = backward || two_resident ? 2 * sm_count : sm_count;
     while (s.ranks < fla::kRecMaxCluster && plan.p.tiles_all * s.ranks * 2 <= most && step() < runs) s.ranks *= 2;
     return s;
   }
@@ -1202,7 +1204,9 @@ Shape shape_of(const Plan& plan, int run_tokens, bool backward, int sm_count) {
 template <typename TX, typename TG, int LPR>
 int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
   constexpr int T = fla::kRunTokens<TX, TG>;
-  Shape shape = shape_of(plan, T, backward, sm_count);
+  constexpr int kFwdBytes = fla::kTileThreads / 32 * fla::kTileSteps * fla::kFwdTile<TX, TG, LPR> + fla::kJoinBytes<LPR>;
+  constexpr bool kTwoResident = kFwdBytes + fla::kTradeBytes<LPR> + 1024 <= 228 * 1024 / 2;
+  Shape shape = shape_of(plan, T, backward, kTwoResident, sm_count);
   const bool alone = plan.p.n <= kShortTokens || plan.farthest > 0x7fffffffLL / (shape.ranks * (shape.threads / LPR) * T);
   long long blocks = plan.p.tiles_all * shape.ranks;
   if (alone) {
@@ -1238,8 +1242,7 @@ int launch(const Plan& plan, bool backward, int sm_count, cudaStream_t stream) {
                               : go(fla::fla_recurrence_bwd_kernel<TX, TG, LPR, 4>, "fla_recurrence_bwd_kernel");
     }
     cfg.blockDim = dim3(fla::kTileThreads + 32);
-    cfg.dynamicSmemBytes = fla::kTileThreads / 32 * fla::kTileSteps * fla::kFwdTile<TX, TG, LPR> + fla::kJoinBytes<LPR> +
-                           (shape.ranks > 1 ? fla::kTradeBytes<LPR> : 0);
+    cfg.dynamicSmemBytes = kFwdBytes + (shape.ranks > 1 ? fla::kTradeBytes<LPR> : 0);
     return plan.piece == 16 ? go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 16>, "fla_recurrence_fwd_kernel")
                             : go(fla::fla_recurrence_fwd_kernel<TX, TG, LPR, 4>, "fla_recurrence_fwd_kernel");
   }
