@@ -6,11 +6,16 @@
 // The reference has no counterpart; its outputs are unnormalised (flashlinear/linear_attn.py:11-31), and a norm of the
 // heads is the usual alternative to the denominator of README.md:27-30.
 //
-// Bound by HBM: a row is read once, into registers, and everything that is summed over it is summed from there (the
-// variance from differences to the mean: no cancellation). A row has a group of 4 to 32 lanes, the smallest whose
-// 16-byte pieces cover it (four to a lane at most), or a CTA where it is longer. Backward, a group adds
-// up its rows' dy n and dy in registers, the groups of a CTA join theirs in shared memory, and a second kernel sums the
-// CTAs'. All orders are fixed.
+// Bound by HBM: a row is read once, and everything that is summed over it is summed from registers (the variance from
+// differences to the mean: no cancellation). A row has a group of 4 to 32 lanes, or whole warps where it is longer; a thread
+// holds 16 of its elements, which shares the shuffles, barriers and addresses of a row among more of them than 8 did
+// (32768 rows of 4096 in bf16, forward: 140 us with 8, 97 with 16). Rows are on their way in shared memory
+// while the ones before are worked on. Backward, a group adds up its rows' dy n and dy in registers, the groups of a CTA join
+// theirs in shared memory, and a second kernel sums the CTAs'. All orders are fixed.
+//
+// Measured (B200, of the 6.45 TB/s of a copy), bf16: 32768 rows of 4096 forward 97 us (86 %), backward 149 (84 %), with a
+// residual 194 (86 %) and 173 (96 %); 1048576 rows of 128 101 (83 %) and 150 (83 %); 524288 rows of 64 in fp16 26 us
+// (79 %). Rows that are no multiple of 16 bytes go element by element: 142848 rows of 83 in fp32 34 (43 %) and 52 (42 %).
 #include <algorithm>
 #include <type_traits>
 

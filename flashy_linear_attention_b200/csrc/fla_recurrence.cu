@@ -5,16 +5,23 @@
 // The reference has no counterpart (its mixers are products of q, k and v, flashlinear/linear_attn.py:11-31).
 //
 // Bound by HBM: two multiply-adds and an exp an element next to 6 bytes (16-bit rows; the backward 10). What it
-// takes is that enough of a sequence is in flight although each step waits for the one before. A step is a map
-// c -> a c + b, and the composition of steps is such a map again, so a run of T tokens is summed from zero
+// takes is that enough of a sequence is in flight although each token waits for the one before. A token is a map
+// c -> a c + b, and the composition of such maps is one again, so a run of T tokens is summed from zero
 // (b) with its decay (a = exp of the sum of its g) without knowing what came before:
-//   * a thread holds two channels of a run of T = 16 tokens (8 with fp32 rows) in registers, read once;
+//   * a thread has two channels of a run of T = 16 tokens (8 where rows or gates are fp32);
 //   * the runs of a CTA exchange (a, b) through shared memory, the CTAs of a cluster, which share a tile of channels
 //     and take neighbouring stretches of tokens, through distributed shared memory, both in one fixed order;
-//   * then each run is walked again from the state before it, out of registers.
-// A cluster walks its sequence from end to end, the rows of the next step being on their way while it
-// exchanges. Nothing is read twice, there is no scratch, no atomic and no wait on memory, and the order of all sums
-// depends on the shapes only.
+//   * then each run is walked again from the state before it.
+// A cluster walks its sequence from end to end, the rows of the next steps being on their way while it
+// exchanges. Nothing is read from memory twice, there is no scratch and no atomic on data, and the order of all sums
+// depends on shapes and strides only. For the backward the forward keeps the state before every run (fp32, 4 and 2.5 % more
+// traffic of the two passes with 16-bit rows), from which the states inside are formed again.
+//
+// Four ways, by what rows allow: short sequences alone in a warp; rows on 16-byte or 4-byte boundaries through tiles in
+// shared memory; 16-bit rows of odd widths by direct loads. Measured (B200, of the 6.45 TB/s of a copy): 4 x 32 heads,
+// 8192 x 128 in bf16 forward 144 us (87 %), backward 233 (89 %); 65536 tokens of 8 x 128 channels with fp32 gates 154 (54 %)
+// and 255 (57 %); 3 x 24 heads, 1984 x 83 in fp32 70 (32 %) and 85 (43 %): the 4-byte copies. Few channels are bound by the time of a
+// step (1.2 us, 1.7 in a cluster of eight), whatever the rows hold: 65536 tokens of 64 channels 71 and 135 us.
 //
 // Accuracy. Channels with a memory of ten thousand tokens multiply the state by exp(-1e-4) as often. That
 // factor rounded to 32 bits is off by up to 3e-8, every time in the same direction. The state is therefore multiplied
@@ -56,7 +63,7 @@ struct RecurrenceParams {
 constexpr int kShortThreads = 128;
 constexpr int kRecMaxCluster = 8;  // (what the exchange holds in registers)
 
-// Tokens a thread holds: a run. 16-bit rows and gates leave room for twice as many.
+// Tokens of a run: what a thread has registers for.
 template <typename TX, typename TG>
 constexpr int kRunTokens = sizeof(TX) + sizeof(TG) <= 4 ? 16 : 8;
 
@@ -306,7 +313,8 @@ __device__ __forceinline__ bool maps_arrived(uint32_t barrier, uint32_t phase, u
 
 // Sends this CTA's map of a step to every CTA of the cluster, itself included, and waits for theirs. The stores count
 // their bytes at the receiver's barrier when they have arrived: unlike a barrier of the cluster, they need no fence, and
-// so do not wait for the rows that were written to memory before (5 us a step that way, 2.5 this way). A peer
+// so do not wait for the rows that were written to memory before (65536 tokens of 64 channels: 348 us that way, 150 this
+// way, with 512 tokens a step). A peer
 // writes to a slot again two steps later, for which it needs what this CTA sends when it has read the slot.
 template <int LPR>
 __device__ __forceinline__ bool trade_maps(const JoinSpace& sh, int step, const RunMap& all, const Team& w,
@@ -982,7 +990,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(con
   const int span = team.ranks * kRuns;                        // runs a step
   const int nth = span - 1 - (team.rank * kRuns + team.run);  // of the step's runs, in the order of the tokens
   const int first = nth / kWarpRuns * kWarpRuns * T, mine = nth % kWarpRuns * T;
-  const TileX xt(p.x, w, column, p.c - column, first), yt(p.o, w, column, p.o.ptr != nullptr ? p.c - column : 0, first);
+  // (a tensor that is not there has no columns: nothing is copied, its rows are zero)
+  const RecurrenceTensor& dy = p.o.ptr != nullptr ? p.o : p.x;
+  const TileX xt(p.x, w, column, p.c - column, first), yt(dy, w, column, p.o.ptr != nullptr ? p.c - column : 0, first);
   const TileX dxt(p.dx, w, column, p.dx.ptr != nullptr ? p.c - column : 0, first);
   const TileG gt(p.g, w, column, p.c - column, first), dgt(p.dg, w, column, p.dg.ptr != nullptr ? p.c - column : 0, first);
   const uint32_t space = shared_address(tiles) + threadIdx.x / 32 * kBwdTile<TX, TG, LPR>;
@@ -995,8 +1005,6 @@ __global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(con
   const int runs_all = (p.n - 1) / T + 1;
   const int steps = (runs_all - 1) / span + 1;
   float2 state;
-  // (a tensor that is not there copies nothing: its rows are zero)
-  const RecurrenceTensor& dy = p.o.ptr != nullptr ? p.o : p.x;
   auto bring = [&](int step) {
     const long long token = static_cast<long long>(step) * span * T;
     const int left = step >= 0 ? static_cast<int>(p.n - token) - first : 0;

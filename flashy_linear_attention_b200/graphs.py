@@ -34,7 +34,9 @@ class CapturedStep:
 
 def capture_step(fn: Callable[[], Any], warmup: int = 2) -> CapturedStep:
     """Runs `fn` `warmup` times on a side stream (so that one-time initialisation and the caching
-    allocator's first allocations happen outside the capture), then captures one call."""
+    allocator's first allocations happen outside the capture), then captures one call. Where `fn` runs a backward pass, no
+    eager graph of the same leaves that was built on the default stream may be alive: autograd would make that stream wait for
+    the captured one, which CUDA refuses."""
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):

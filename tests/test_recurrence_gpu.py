@@ -353,6 +353,22 @@ def test_far_offsets():
     check("s_final", s_final, want["s_final"])
 
 
+@pytest.mark.parametrize("N,apart", [(40, 2**26), (8192, 2**18)])
+def test_offsets_past_32_bits(N, apart):
+    """Rows that are read and written 2^26 elements apart (a step's offsets pass 32 bits) and 2^18 (those of the sequence do)."""
+    far = [torch.empty(N * apart, dtype=BF, device=DEV).as_strided((1, 1, N, 64), (0, 0, apart, 1)) for _ in range(2)]
+    x, g, s, dy, ds = make(1, 1, N, 64)
+    far[0].copy_(x)
+    far[1].copy_(dy)
+    want = run(x, g, s, dy, ds)
+    got = run(far[0], g, s, far[1], ds)
+    ref = reference(x[:, :, :40], g[:, :, :40], s)
+    check("out", got["out"][:, :, :40], ref["out"])
+    for name in got:  # (the same sums in another order where the step is another)
+        off, size = (got[name].double() - want[name].double()).norm(), want[name].double().norm()  # (zero behind a reset)
+        assert off <= (torch.finfo(got[name].dtype).eps + 1e-5) * size, name
+
+
 def test_the_same_bits_every_time():
     for shape in ((1, 2, 2000, 64), (4, 40, 300, 64), (2, 3, 500, 83)):
         t = make(*shape)
