@@ -35,10 +35,12 @@ struct LayerNormParams {
   const void* w;          // [heads][d] or null
   const void* b;
   int w_wide;             // weights are fp32 (else of the rows' type)
-  float* stats;           // [heads][rows][2]: mean, r; null: not wanted (forward)
+  float* stats;           // [heads][rows][2]: mean, r, rows in the order of their indices; null: not wanted (forward)
   float* parts;           // backward: [CTA][2][heads][d], or null
   long long rows;         // of a head
   int heads, n1, n2, d;   // row j is (j / n2 / n1, j / n2 % n1, j % n2)
+  int stat_n1, stat_n2;   // n1 and n2 of the indices that stat_step belongs to; stat_n2 0: row j has its statistics at j
+  unsigned stat_step[3];
   int lanes;              // threads that share a row, where they are whole warps
   float eps;
 };
@@ -73,6 +75,17 @@ struct Cursor {
     if (FLAT) at += step_bytes;
   }
 };
+
+// Where the statistics of row j are. They go by the rows' indices and not by where these lie, since a tensor that is kept
+// for the backward can come back with other strides.
+__device__ __forceinline__ float* stats_of(const LayerNormParams& p, int head, unsigned j) {
+  if (p.stat_n2 != 0) {
+    const unsigned outer = j / static_cast<unsigned>(p.stat_n2), i2 = j - outer * p.stat_n2;
+    const unsigned i0 = outer / static_cast<unsigned>(p.stat_n1), i1 = outer - i0 * p.stat_n1;
+    j = i0 * p.stat_step[0] + i1 * p.stat_step[1] + i2 * p.stat_step[2];
+  }
+  return p.stats + 2 * (head * p.rows + j);
+}
 
 // A piece of a row: 16 bytes, or one element where rows are not aligned or end inside a piece.
 template <typename T, bool WIDE>
@@ -419,7 +432,7 @@ fla_layer_norm_fwd_kernel(const LayerNormParams p) {
       const unsigned row = j + r * stride;
       const float root = reciprocal_root(fmaf(sum[r], over_d, p.eps));
       if (p.stats != nullptr && t.lane == 0 && row < rows)
-        *reinterpret_cast<float2*>(p.stats + 2 * (head * p.rows + row)) = make_float2(mean[r], root);
+        *reinterpret_cast<float2*>(stats_of(p, head, row)) = make_float2(mean[r], root);
 #pragma unroll
       for (int i = 0; i < P; ++i) v[r][i] = fma2(mul2(v[r][i], both(root)), w[i], b[i]);
       Regs y;
@@ -473,7 +486,7 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
     next += stride;
   };
   auto fetch_stats = [&] {
-    stats = stats_next < rows ? __ldg(reinterpret_cast<const float2*>(p.stats + 2 * (head * p.rows + stats_next))) : both(0.f);
+    stats = stats_next < rows ? __ldg(reinterpret_cast<const float2*>(stats_of(p, head, stats_next))) : both(0.f);
     stats_next += stride;
   };
   float2* const sums_at = reinterpret_cast<float2*>(reinterpret_cast<char*>(slots) + (Ahead::kStaged ? 3 * Ahead::kDepth * Ahead::kBytes * blockDim.x : 0)) + threadIdx.x;
@@ -672,16 +685,23 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
   p.eps = a->eps;
   NormRows* const used[] = {&p.x, backward ? &p.dy : &p.y, backward ? &p.dx : &p.s, backward ? &p.ds : &p.z};
   long long n0 = a->batch;
-  // Rows are numbered as they lie in memory in what is normalised (the same tensor in both passes, whatever the others
-  // look like: `stats` goes by these numbers).
+  // Rows are numbered as they lie in memory in what is normalised.
   const NormRows order = backward || p.s.ptr == nullptr ? p.x : p.s;
+  p.stat_step[0] = p.n1 * p.n2;
+  p.stat_step[1] = p.n2;
+  p.stat_step[2] = 1;
+  bool moved = false;  // a dim of several rows before another
   auto swap01 = [&] {
+    moved = moved || (n0 > 1 && p.n1 > 1);
+    std::swap(p.stat_step[0], p.stat_step[1]);
     for (NormRows* t : used) std::swap(t->s0, t->s1);
     const int n = static_cast<int>(n0);
     n0 = p.n1;
     p.n1 = n;
   };
   auto swap12 = [&] {
+    moved = moved || (p.n1 > 1 && p.n2 > 1);
+    std::swap(p.stat_step[1], p.stat_step[2]);
     for (NormRows* t : used) std::swap(t->s1, t->s2);
     std::swap(p.n1, p.n2);
   };
@@ -691,6 +711,8 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
     if (s2 > s1) swap12(), std::swap(s1, s2);
     if (s1 > s0) swap01();
   }
+  p.stat_n1 = p.n1;
+  p.stat_n2 = moved ? p.n2 : 0;
   // neighbouring dims that are one in every tensor
   auto every = [&](auto&& holds) {
     for (NormRows* t : used)

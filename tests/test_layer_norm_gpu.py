@@ -174,6 +174,19 @@ def test_ranks_and_strides():
     verify(turned, None, wide[0, 1:], wide[1, 1:].contiguous(), dy, None)
 
 
+@pytest.mark.parametrize("shape,order", [((3, 5, 70, 64), (0, 2, 1, 3)), ((3, 5, 70, 64), (2, 1, 0, 3)), ((3, 5, 70, 64), (1, 2, 0, 3)),
+                                         ((2, 1, 33, 83), (2, 0, 1, 3)), ((3, 40, 128), (1, 0, 2)), ((2, 3, 4, 5, 32), (1, 3, 2, 0, 4))])
+@pytest.mark.parametrize("add", [False, True])
+def test_kept_tensors_that_come_back_with_other_strides(shape, order, add):
+    """What autograd keeps can be packed away and unpacked contiguous; rows in memory order `order` (from outside in)."""
+    x, z, w, b, dy, ds = make(shape)
+    back = [order.index(i) for i in range(len(order))]
+    x, z = (t.permute(order).contiguous().permute(back) for t in (x, z))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.contiguous()):
+        verify(x, z if add else None, w, b, dy, ds)
+    verify(x, z if add else None, w, b, dy, ds)
+
+
 @pytest.mark.parametrize("shape,heads", [((2, 9, 96), False), ((2, 3, 9, 96), True), ((4, 2048), False)])
 def test_without_weights_and_some_gradients_only(shape, heads):
     LayerNorm, AddLayerNorm = functions()
