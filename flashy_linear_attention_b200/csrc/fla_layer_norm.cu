@@ -29,6 +29,15 @@ struct NormRows {
   long long sh, s0, s1, s2;  // bytes: from head to head (weights of the heads' own), and in the three dims of the rows
 };
 
+// Exact division of numbers below 2^31 by one that the host knows: with l = ceil(log2 d) and mul = floor(2^(31 + l) / d) + 1,
+// mul d is above 2^(31 + l) by 2^l at most, so j mul / 2^(31 + l) is above j / d by less than 1 / d.
+struct Divisor {
+  unsigned d, mul, shift;
+};
+__device__ __forceinline__ unsigned over(unsigned j, const Divisor& d) {
+  return static_cast<unsigned>(static_cast<unsigned long long>(j) * d.mul >> d.shift);
+}
+
 struct LayerNormParams {
   NormRows x, z, s, y;    // forward: rows, residual (null: none), their sum (output), result
   NormRows dy, ds, dx;    // backward: x is what was normalised; ds null: none; dx null: not wanted
@@ -39,14 +48,15 @@ struct LayerNormParams {
   float* parts;           // backward: [CTA][2][heads][d], or null
   long long rows;         // of a head
   int heads, n1, n2, d;   // row j is (j / n2 / n1, j / n2 % n1, j % n2)
-  int stat_n1, stat_n2;   // n1 and n2 of the indices that stat_step belongs to; stat_n2 0: row j has its statistics at j
+  Divisor by_n1, by_n2;
+  Divisor stat_n1, stat_n2;  // not FLAT: row j has its statistics at the place that its indices have with these steps
   unsigned stat_step[3];
   int lanes;              // threads that share a row, where they are whole warps
   float eps;
 };
 
 // The rows that a group of threads works on, one after the other: their numbers are `step` apart. FLAT: all rows of a head
-// are one stride apart in every tensor, and addresses are advanced, not worked out (64-bit products and a division for
+// are one stride apart in every tensor, in the order of their indices, and addresses are advanced, not worked out (64-bit products and a division for
 // each row and tensor were a third of the instructions).
 template <bool FLAT>
 struct Cursor {
@@ -67,8 +77,8 @@ struct Cursor {
   __device__ __forceinline__ char* get(const LayerNormParams& p, unsigned row, bool in) const {
     if (FLAT) return at;
     if (!in) return t->ptr;
-    const unsigned outer = row / static_cast<unsigned>(p.n2), i2 = row - outer * p.n2;
-    const unsigned i0 = outer / static_cast<unsigned>(p.n1), i1 = outer - i0 * p.n1;
+    const unsigned outer = over(row, p.by_n2), i2 = row - outer * p.n2;
+    const unsigned i0 = over(outer, p.by_n1), i1 = outer - i0 * p.n1;
     return t->ptr + (of_head + i0 * t->s0 + i1 * t->s1 + i2 * t->s2);
   }
   __device__ __forceinline__ void advance() {
@@ -78,11 +88,11 @@ struct Cursor {
 
 // Where the statistics of row j are. They go by the rows' indices and not by where these lie, since a tensor that is kept
 // for the backward can come back with other strides.
+template <bool FLAT>
 __device__ __forceinline__ float* stats_of(const LayerNormParams& p, int head, unsigned j) {
-  if (p.stat_n2 != 0) {
-    const unsigned outer = j / static_cast<unsigned>(p.stat_n2), i2 = j - outer * p.stat_n2;
-    const unsigned i0 = outer / static_cast<unsigned>(p.stat_n1), i1 = outer - i0 * p.stat_n1;
-    j = i0 * p.stat_step[0] + i1 * p.stat_step[1] + i2 * p.stat_step[2];
+  if (!FLAT) {
+    const unsigned outer = over(j, p.stat_n2), i0 = over(outer, p.stat_n1);
+    j = i0 * p.stat_step[0] + (outer - i0 * p.stat_n1.d) * p.stat_step[1] + (j - outer * p.stat_n2.d) * p.stat_step[2];
   }
   return p.stats + 2 * (head * p.rows + j);
 }
@@ -432,7 +442,7 @@ fla_layer_norm_fwd_kernel(const LayerNormParams p) {
       const unsigned row = j + r * stride;
       const float root = reciprocal_root(fmaf(sum[r], over_d, p.eps));
       if (p.stats != nullptr && t.lane == 0 && row < rows)
-        *reinterpret_cast<float2*>(stats_of(p, head, row)) = make_float2(mean[r], root);
+        *reinterpret_cast<float2*>(stats_of<FLAT>(p, head, row)) = make_float2(mean[r], root);
 #pragma unroll
       for (int i = 0; i < P; ++i) v[r][i] = fma2(mul2(v[r][i], both(root)), w[i], b[i]);
       Regs y;
@@ -486,7 +496,7 @@ fla_layer_norm_bwd_kernel(const LayerNormParams p) {
     next += stride;
   };
   auto fetch_stats = [&] {
-    stats = stats_next < rows ? __ldg(reinterpret_cast<const float2*>(stats_of(p, head, stats_next))) : both(0.f);
+    stats = stats_next < rows ? __ldg(reinterpret_cast<const float2*>(stats_of<FLAT>(p, head, stats_next))) : both(0.f);
     stats_next += stride;
   };
   float2* const sums_at = reinterpret_cast<float2*>(reinterpret_cast<char*>(slots) + (Ahead::kStaged ? 3 * Ahead::kDepth * Ahead::kBytes * blockDim.x : 0)) + threadIdx.x;
@@ -661,6 +671,12 @@ NormRows norm_rows(const FlaTensor& t, int size, bool heads_apart) {
   return r;
 }
 
+fla::Divisor divisor(int d) {
+  unsigned l = 0;
+  while ((1LL << l) < d) ++l;
+  return {static_cast<unsigned>(d), static_cast<unsigned>((1ULL << (31 + l)) / d + 1), 31 + l};
+}
+
 NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
   NormPlan plan = {};
   LayerNormParams& p = plan.p;
@@ -711,8 +727,8 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
     if (s2 > s1) swap12(), std::swap(s1, s2);
     if (s1 > s0) swap01();
   }
-  p.stat_n1 = p.n1;
-  p.stat_n2 = moved ? p.n2 : 0;
+  p.stat_n1 = divisor(p.n1);
+  p.stat_n2 = divisor(p.n2);
   // neighbouring dims that are one in every tensor
   auto every = [&](auto&& holds) {
     for (NormRows* t : used)
@@ -740,7 +756,9 @@ NormPlan norm_plan(const FlaLayerNormArgs* a, bool backward, int sm_count) {
     for (NormRows* t : used) t->s1 = t->s0;
   }
   const int per = 16 / size;
-  plan.flat = p.n1 == 1 && p.rows == p.n2;
+  p.by_n1 = divisor(p.n1);
+  p.by_n2 = divisor(p.n2);
+  plan.flat = !moved && p.n1 == 1 && p.rows == p.n2;
   auto aligned = [](const void* q, int n) { return reinterpret_cast<uintptr_t>(q) % n == 0; };
   plan.wide = p.d % per == 0 && aligned(p.w, 16) && aligned(p.b, 16) && every([&](const NormRows& t) {
                 return aligned(t.ptr, 16) && (p.heads == 1 || t.sh % 16 == 0) && (n0 == 1 || t.s0 % 16 == 0) &&
