@@ -1218,7 +1218,7 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward, int sm_count) {
   plan.piece = plan.pair && rows_on(16) ? 16 : rows_on(4) ? 4 : 0;
   plan.farthest = 1;
   every([&](const RecurrenceTensor& t, int size) {
-    plan.farthest = std::max(plan.farthest, t.sn * size);
+    plan.farthest = std::max(plan.farthest, t.sn < 0 ? INT64_MAX : t.sn * size);  // (backwards: alone, too, where offsets have a sign)
     return true;
   });
   // Tiles of 64 columns; of 32 where that leaves fewer lanes without one, and for few channels, whose clusters of eight would
@@ -1320,8 +1320,8 @@ int check(const FlaRecurrenceArgs* a) {
   if (a == nullptr || a->batch <= 0 || a->heads <= 0 || a->seqlen <= 0 || a->dim <= 0) return FLA_ERR_INVALID;
   if (!known_type(a->dtype) || (a->g_dtype != a->dtype && a->g_dtype != FLA_DTYPE_F32)) return FLA_ERR_INVALID;
   if (a->x.ptr == nullptr || a->g.ptr == nullptr) return FLA_ERR_INVALID;
-  // run and token numbers are 32-bit, a step past the end included
-  if (a->seqlen > (1 << 30) || static_cast<long long>(a->batch) * a->heads > (1 << 30)) return FLA_ERR_UNSUPPORTED;
+  // run, token and column numbers are 32-bit, a step or a tile past the end included
+  if (a->seqlen > (1 << 30) || a->dim > (1 << 30) || static_cast<long long>(a->batch) * a->heads > (1 << 30)) return FLA_ERR_UNSUPPORTED;
   const int x = element_bytes(a->dtype), g = element_bytes(a->g_dtype);
   auto off = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
   if (off(a->x.ptr, x) || off(a->o.ptr, x) || off(a->d_o.ptr, x) || off(a->d_x.ptr, x) || off(a->g.ptr, g) ||

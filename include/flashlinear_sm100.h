@@ -346,8 +346,9 @@ int fla_sm100_taylor_bwd(const FlaArgs* args);
 /* ---- gated linear recurrence ----
  * h_t = exp(g_t) h_(t-1) + x_t for every channel of [batch, heads, seqlen, dim] tensors, out_t = h_t. g_t = -inf drops the
  * state, whatever it holds (a document starts); g_t = 0 and x_t = 0 leave it as it is (a token to be passed over).
- * The reference has no counterpart. Tensors have any (batch, head, token) strides, zero for broadcast inputs included,
- * and an innermost stride of 1; nothing has to be aligned beyond its element size. States are fp32
+ * The reference has no counterpart. Tensors have any (batch, head, token) strides, zero for broadcast inputs and negative
+ * ones included, and an innermost stride of 1; nothing has to be aligned beyond its element size; seqlen, dim and
+ * batch * heads are up to 2^30. States are fp32
  * [batch, heads, dim], contiguous. dtype is that of x, o, d_o and d_x, g_dtype that of g and d_g: the same or fp32.
  * fwd reads x, g and s_init (null: zero), writes o and, unless null, s_final and `states`: the state before every
  * few tokens, of recurrence_states_bytes(), 16-byte aligned, private to the library, for the backward of the same x and g.

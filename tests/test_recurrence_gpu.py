@@ -369,6 +369,25 @@ def test_offsets_past_32_bits(N, apart):
         assert off <= (torch.finfo(got[name].dtype).eps + 1e-5) * size, name
 
 
+@pytest.mark.parametrize("N", [5, 700])
+def test_negative_strides(N):
+    """Tokens from the last to the first, which the C interface can be given."""
+    from flashy_linear_attention_b200 import recurrence as rec
+
+    x, g, s, _, _ = make(2, 3, N, 64)
+    out, s_final = torch.empty_like(x), torch.empty_like(s)
+    a = rec._args(x, g)
+    a.o = rec._desc(out)
+    for t, of in ((a.x, x), (a.g, g), (a.o, out)):
+        t.ptr += (N - 1) * of.stride(2) * of.element_size()
+        t.stride_n = -of.stride(2)
+    a.s_init, a.s_final = s.data_ptr(), s_final.data_ptr()
+    rec._call("fla_sm100_recurrence_fwd", a, x.device)
+    want = reference(x.flip(2), g.flip(2), s)
+    check("out", out.flip(2), want["out"])
+    check("s_final", s_final, want["s_final"])
+
+
 def test_the_same_bits_every_time():
     for shape in ((1, 2, 2000, 64), (4, 40, 300, 64), (2, 3, 500, 83)):
         t = make(*shape)

@@ -85,6 +85,7 @@ def test_c_interface_refuses():
     assert fwd(args(dtype=3)) == -1 and fwd(args(g_dtype=1)) == -1 and fwd(args(dtype=2, g_dtype=0)) == -1
     assert fwd(args(x=odd)) == -3 and bwd(args(d_g=odd)) == -3 and fwd(args(s_init=66)) == -3 and fwd(args(states=68)) == -3
     assert fwd(args(seqlen=(1 << 30) + 1)) == -2 and fwd(args(batch=1 << 20, heads=1 << 20)) == -2
+    assert fwd(args(dim=(1 << 30) + 1)) == -2 and bwd(args(dim=2**31 - 1, states_bytes=1 << 40)) == -2
     # the state before every 16 tokens, 8 where a row or the gates are fp32
     assert size(args()) == 4 * 2 * 3 * 8 * 3 and size(args(g_dtype=2)) == 4 * 2 * 3 * 8 * 5
     assert fwd(args(states_bytes=575)) == -5 and bwd(args(states_bytes=575)) == -5 and bwd(args(states=None)) == -5
