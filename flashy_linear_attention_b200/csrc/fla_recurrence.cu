@@ -138,7 +138,9 @@ __device__ __forceinline__ float2 advance(float2 g, float2 h, float2 x) {
   }
   return r;
 }
-// The same step backward: exp(g) times what has come together at the token.
+// The same step backward, R_t = exp(g) G_t. The backward kernels carry G and not R from token to token, G_t = dO_t +
+// exp(g_(t+1)) G_(t+1) in one operation wherever it is formed: as a product and a sum it is compiled to one in some of the walks
+// and to two in others, and the bits of a channel then depend on whether another one's gates call for a careful walk.
 template <typename TX, bool DROPS>
 __device__ __forceinline__ float2 retreat(float2 g, float2 all) {
   float2 r = mul2(decay<TX>(g), all);
@@ -490,12 +492,17 @@ __device__ __noinline__ float2 advance_from(float2 h, const typename PairOf<TX>:
   }
   return h;
 }
+// R before a run from zero behind it, with what a gate of minus infinity drops left out.
 template <typename TX, typename TG, int T>
 __device__ __noinline__ float2 retreat_from_zero(const typename PairOf<TX>::Raw* y, const typename PairOf<TG>::Raw* g) {
-  float2 r = make_float2(0.f, 0.f);
+  float2 all = make_float2(0.f, 0.f), gate = all;  // gate: the one behind the token
 #pragma unroll 1
-  for (int t = T - 1; t >= 0; --t) r = retreat<TX, true>(unpack_pair<TG>(g[t]), add2(unpack_pair<TX>(y[t]), r));
-  return r;
+  for (int t = T - 1; t >= 0; --t) {
+    const float2 yv = unpack_pair<TX>(y[t]);
+    all = t == T - 1 ? yv : advance<TX, true>(gate, all, yv);
+    gate = unpack_pair<TG>(g[t]);
+  }
+  return retreat<TX, true>(gate, all);
 }
 template <typename R, int T>
 struct InMemory {
@@ -632,13 +639,15 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_
   if (team.ranks > 1) cg::this_cluster().sync();  // every CTA has started before a peer writes to it
   // The walk starts at the end; the runs behind the last token are the identity. Steps before the last one are whole.
   for (int step = steps - 1; step >= 0; --step) {
-    float2 sum = make_float2(0.f, 0.f), r = sum, h = state;
+    float2 sum = make_float2(0.f, 0.f), r = sum, a = sum, h = state;
 #pragma unroll
     for (int t = T - 1; t >= 0; --t) {
       const float2 gv = unpack_pair<TG>(g[t]);
       sum = add2(sum, gv);
-      r = retreat<TX, false>(gv, add2(unpack_pair<TX>(y[t]), r));
+      r = t == T - 1 ? unpack_pair<TX>(y[t]) : fma2(a, r, unpack_pair<TX>(y[t]));
+      a = decay<TX>(gv);
     }
+    r = mul2(a, r);
     const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
     float2 before[T];  // the state before each token
     anew(g);
@@ -677,22 +686,26 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_
       const char *ys = yr.step(p.o, token - static_cast<long long>(span) * T), *gs = gr.step(p.g, token - static_cast<long long>(span) * T);
 #pragma unroll
       for (int t = T - 1; t >= 0; --t) {
-        const float2 all = add2(unpack_pair<TX>(y[t]), r);
+        const float2 all = t == T - 1 ? add2(unpack_pair<TX>(y[t]), r) : fma2(a, r, unpack_pair<TX>(y[t]));
         dxr.store(dxs, t, w, all);
-        r = retreat<TX, false>(unpack_pair<TG>(g[t]), all);
-        dgr.store(dgs, t, w, mul2(r, before[t]));
+        a = decay<TX>(unpack_pair<TG>(g[t]));
+        dgr.store(dgs, t, w, mul2(mul2(a, all), before[t]));
+        r = all;
         y[t] = yr.load(ys, t, r.x);
         g[t] = gr.load(gs, t, r.x);
       }
     } else {
+      float2 gate = make_float2(0.f, 0.f);  // the one behind the token
 #pragma unroll
       for (int t = T - 1; t >= 0; --t) {
-        const float2 gv = unpack_pair<TG>(g[t]), all = add2(unpack_pair<TX>(y[t]), r);
+        const float2 gv = unpack_pair<TG>(g[t]), yv = unpack_pair<TX>(y[t]);
+        const float2 all = t == T - 1 ? add2(yv, r) : advance<TX, true>(gate, r, yv);
         const bool in = token + first + t < p.n;
         if (in && want_dx) dxr.store(dxs, t, w, all);
-        r = retreat<TX, true>(gv, all);
+        r = all;
+        gate = gv;
         if (in && want_dg) {
-          float2 d = mul2(r, before[t]);
+          float2 d = mul2(mul2(decay<TX>(gv), all), before[t]);
           if (gv.x == -INFINITY) d.x = 0.f;
           if (gv.y == -INFINITY) d.y = 0.f;
           dgr.store(dgs, t, w, d);
@@ -823,21 +836,6 @@ __device__ __forceinline__ void copies_wait() {
 // of the time: 377 us without, 449 with them).
 __device__ __forceinline__ bool spoilt(bool drops, float2 v) {
   return drops && __any_sync(0xffffffffu, !(fabsf(v.x) <= 3.4e38f && fabsf(v.y) <= 3.4e38f));
-}
-
-// R before a run from zero behind it, with what a gate of minus infinity (or one whose decay is zero) drops left out.
-template <typename TX, typename TG, int T>
-__device__ __noinline__ float2 retreat_with_care(const typename PairOf<TX>::Raw* y, const typename PairOf<TG>::Raw* g) {
-  float2 all = make_float2(0.f, 0.f), a = all;
-#pragma unroll 1
-  for (int t = T - 1; t >= 0; --t) {
-    const float2 yv = unpack_pair<TX>(y[t]);
-    all = t == T - 1 ? yv : fma2(a, all, yv);
-    if (t < T - 1 && a.x == 0.f) all.x = yv.x;
-    if (t < T - 1 && a.y == 0.f) all.y = yv.y;
-    a = decay<TX>(unpack_pair<TG>(g[t]));
-  }
-  return make_float2(a.x == 0.f ? 0.f : a.x * all.x, a.y == 0.f ? 0.f : a.y * all.y);
 }
 
 // Forward, eight warps work on runs and a ninth joins them, a step apart: while it joins the runs of one step, the others sum those
@@ -1051,7 +1049,6 @@ __global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(con
     typename PairOf<TG>::Raw g[T];
     copies_wait<0>();
     float2 sum = make_float2(0.f, 0.f), r = sum, h = state;
-    // (G_t = dy_t + a_(t+1) G_(t+1) as one operation in all three places, or those that are walked with care round otherwise)
     float2 a = sum;
 #pragma unroll
     for (int t = T - 1; t >= 0; --t) {
@@ -1074,7 +1071,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(con
     if (spoilt(drops, r)) {
       const InMemory<typename PairOf<TX>::Raw, T> ym(y);
       const InMemory<typename PairOf<TG>::Raw, T> gm(g);
-      r = retreat_with_care<TX, TG, T>(ym.v, gm.v);
+      r = retreat_from_zero<TX, TG, T>(ym.v, gm.v);
     }
     const bool states_spoilt = spoilt(drops, h);
     if (states_spoilt) {
@@ -1111,14 +1108,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(con
 #pragma unroll 1
       for (int t = T - 1; t >= 0; --t) {
         const float2 yv = unpack_pair<TX>(ym.v[t]), gv = unpack_pair<TG>(gm.v[t]);
-        float2 all = t == T - 1 ? add2(yv, r) : fma2(a, r, yv);
-        if (t < T - 1 && a.x == 0.f) all.x = yv.x;
-        if (t < T - 1 && a.y == 0.f) all.y = yv.y;
+        const float2 all = t == T - 1 ? add2(yv, r) : advance<TX, true>(unpack_pair<TG>(gm.v[t + 1]), r, yv);
         TileX::put(dx_at + x_run, t, all);
-        a = decay<TX>(gv);
-        float2 d = mul2(mul2(a, all), bm.v[t]);
-        if (a.x == 0.f) d.x = 0.f;
-        if (a.y == 0.f) d.y = 0.f;
+        float2 d = mul2(mul2(decay<TX>(gv), all), bm.v[t]);
+        if (gv.x == -INFINITY) d.x = 0.f;
+        if (gv.y == -INFINITY) d.y = 0.f;
         TileG::put(dg_at + g_run, t, d);
         r = all;
       }
