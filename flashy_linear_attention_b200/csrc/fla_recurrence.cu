@@ -151,6 +151,15 @@ __device__ __forceinline__ float2 retreat(float2 g, float2 all) {
   return r;
 }
 
+// Whether a run drops the state is read from the sum of its gates, which is minus infinity then, unless a NaN or plus infinity
+// among them made it NaN: a run with such a sum is looked through (mark_drops), and its sum is minus infinity again from there on.
+__device__ __forceinline__ bool may_drop(float2 sum) { return !(sum.x > -INFINITY && sum.y > -INFINITY); }
+__device__ __forceinline__ bool no_number(float2 sum) { return sum.x != sum.x || sum.y != sum.y; }
+__device__ __forceinline__ void mark_drops(float2 gate, float2* sum) {
+  if (gate.x == -INFINITY) sum->x = -INFINITY;
+  if (gate.y == -INFINITY) sum->y = -INFINITY;
+}
+
 struct Place {  // what a thread works on
   int b, h, c0, gap;
   bool ok0, ok1;
@@ -372,6 +381,13 @@ __device__ __forceinline__ void join(const JoinSpace& sh, int step, const Team& 
         b = apply_map(b, m[i]);
       }
     }
+    if (no_number(sum)) {  // (one run's NaN hides that another drops)
+#pragma unroll 1
+      for (int i = 0; i < RUNS; ++i) {
+        const float2 hi = sh.run[i * LPR + w.lane].hi;
+        mark_drops(make_float2(hi.x < 0.f ? -INFINITY : 0.f, hi.y < 0.f ? -INFINITY : 0.f), &sum);
+      }
+    }
     if (!lost && !trade_maps<LPR>(sh, step, run_map(sum, b), w, p)) {
       lost = true;
       if (p.status != nullptr) atomicOr(p.status, 1);
@@ -504,6 +520,12 @@ __device__ __noinline__ float2 retreat_from_zero(const typename PairOf<TX>::Raw*
   }
   return retreat<TX, true>(gate, all);
 }
+template <typename TG, int T>
+__device__ __noinline__ float2 sum_with_drops(float2 sum, const typename PairOf<TG>::Raw* g) {
+#pragma unroll 1
+  for (int t = 0; t < T; ++t) mark_drops(unpack_pair<TG>(g[t]), &sum);
+  return sum;
+}
 template <typename R, int T>
 struct InMemory {
   R v[T];
@@ -552,10 +574,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fla_recurrence_direct
       sum = add2(sum, gv);
       h = advance<TX, false>(gv, h, unpack_pair<TX>(x[t]));
     }
-    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    const bool drops = __any_sync(0xffffffffu, may_drop(sum));
     if (drops) {
       const InMemory<typename PairOf<TX>::Raw, T> xm(x);
       const InMemory<typename PairOf<TG>::Raw, T> gm(g);
+      if (__any_sync(0xffffffffu, no_number(sum))) sum = sum_with_drops<TG, T>(sum, gm.v);
       h = advance_from<TX, TG, T>(make_float2(0.f, 0.f), xm.v, gm.v, nullptr);
     }
     h = exchange(sh, step, sum, h, team, p, carry, lost);
@@ -648,13 +671,14 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) fla_recurrence_direct_
       a = decay<TX>(gv);
     }
     r = mul2(a, r);
-    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    const bool drops = __any_sync(0xffffffffu, may_drop(sum));
     float2 before[T];  // the state before each token
     anew(g);
     if (drops) {
       const InMemory<typename PairOf<TX>::Raw, T> xm(x), ym(y);
       const InMemory<typename PairOf<TG>::Raw, T> gm(g);
       float2 bm[T];
+      if (__any_sync(0xffffffffu, no_number(sum))) sum = sum_with_drops<TG, T>(sum, gm.v);
       r = retreat_from_zero<TX, TG, T>(ym.v, gm.v);
       advance_from<TX, TG, T>(h, xm.v, gm.v, bm);
 #pragma unroll
@@ -924,7 +948,7 @@ __global__ void __launch_bounds__(kTileThreads + 32, 2) fla_recurrence_fwd_kerne
       gt.copy(tile + TileX::kBytes, gt.step(p.g, token), left);
       copies_end();
     };
-    // The first walk: the run's sum from zero, and of its gates. True where one of them is minus infinity.
+    // The first walk: the run's sum from zero, and of its gates. True where one of them may be minus infinity.
     auto sum_up = [&](int step, uint32_t tile) {
       float2 sum = make_float2(0.f, 0.f), h = sum;
 #pragma unroll
@@ -933,7 +957,11 @@ __global__ void __launch_bounds__(kTileThreads + 32, 2) fla_recurrence_fwd_kerne
         sum = add2(sum, gv);
         h = fma2(decay<TX>(gv), h, unpack_pair<TX>(TileX::get(tile + x_run, t)));
       }
-      const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+      const bool drops = __any_sync(0xffffffffu, may_drop(sum));
+      if (drops && __any_sync(0xffffffffu, no_number(sum))) {
+#pragma unroll 1
+        for (int t = 0; t < T; ++t) mark_drops(unpack_pair<TG>(TileG::get(tile + g_run, t)), &sum);
+      }
       if (spoilt(drops, h)) {
         h = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -1060,7 +1088,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) fla_recurrence_bwd_kernel(con
       a = decay<TX>(gv);
     }
     r = mul2(a, r);
-    const bool drops = __any_sync(0xffffffffu, sum.x == -INFINITY || sum.y == -INFINITY);
+    const bool drops = __any_sync(0xffffffffu, may_drop(sum));
+    if (drops && __any_sync(0xffffffffu, no_number(sum))) {
+#pragma unroll 1
+      for (int t = 0; t < T; ++t) mark_drops(unpack_pair<TG>(TileG::get(g_at + g_run, t)), &sum);
+    }
     float2 before[T];  // the state before each token
     anew(g);
 #pragma unroll

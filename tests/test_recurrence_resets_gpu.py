@@ -58,6 +58,28 @@ def others(got, want, channel, what):
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 @pytest.mark.parametrize("N,resets", [(20, (1, 9, 19)), (400, (7, 100, 399)), (5000, (513, 2503))])
+def test_no_gate_reaches_past_a_reset(kind, N, resets):
+    for at in resets:
+        x, g, s, dy, ds = make(N, *kind, seed=at)
+        g[:, :, at] = -math.inf
+        clean = run(x, g, s, dy, ds)
+        for poison in (math.nan, math.inf):
+            for away in (1, 2, 5, 40, 300):  # in the same run, in others of a CTA, in another CTA
+                for at_gate in (at - away, at + away):
+                    if not 0 <= at_gate < N:
+                        continue
+                    what = f"gate {at_gate} {poison}, reset {at}"
+                    bad = g.clone()
+                    bad[:, :, at_gate] = poison
+                    got = run(x, bad, s, dy, ds)
+                    (after if at_gate < at else before)(got, clean, at, what)
+                    bad = g.clone()
+                    bad[..., at_gate, 3] = poison
+                    others(run(x, bad, s, dy, ds), clean, 3, what)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("N,resets", [(20, (1, 9, 19)), (400, (7, 100, 399)), (5000, (513, 2503))])
 def test_nothing_passes_a_reset_in_any_kernel(kind, N, resets):
     for at in resets:
         x, g, s, dy, ds = make(N, *kind, seed=at)
