@@ -243,6 +243,10 @@ class TaylorLinearAttention(Function):
         return ops.taylor_backward_in_memory(grad_output, xq, xk, v, *features)
 
 
+# The Functions below take a native autograd node where there is one that covers the call, and else the Python Function of the same
+# name with an underscore. That one is called by its name: torch.compile can trace this, but no super().apply of a Function.
+
+
 def _native_node(x):
     """The native host path, for Functions that have a node there. Not with FLA_DEBUG=1, where the status is read after every
     call, the backward's included."""
@@ -251,7 +255,25 @@ def _native_node(x):
     return _lib.host()
 
 
-class GatedLinearRecurrence(Function):
+class _GatedLinearRecurrence(Function):
+    @staticmethod
+    def forward(ctx: Any, x, log_decay, s_init=None):
+        out, s_final, states = recurrence.recurrence_fwd(x, log_decay, s_init, any(ctx.needs_input_grad[:3]))
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, log_decay, states)
+        return out, s_final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_output, grad_s_final):
+        x, log_decay, states = ctx.saved_tensors
+        if grad_output is None and grad_s_final is None:
+            return None, None, None
+        needs = tuple(ctx.needs_input_grad) + (False,) * (3 - len(ctx.needs_input_grad))
+        return tuple(recurrence.recurrence_bwd(grad_output, x, log_decay, states, grad_s_final, needs)[:len(ctx.needs_input_grad)])
+
+
+class GatedLinearRecurrence(_GatedLinearRecurrence):
     """Gated linear recurrence, a state of its own for every channel:
     ``h_t = exp(log_decay_t) h_{t-1} + x_t``, ``out_t = h_t``.
 
@@ -275,29 +297,28 @@ class GatedLinearRecurrence(Function):
             x = x.to(torch.bfloat16)
             if log_decay.dtype != torch.float32:
                 log_decay = log_decay.to(torch.bfloat16)
-        # (a native autograd node, which the forward and backward below stand in for where it does not cover the call)
+        # (a native autograd node, for which the Python Function above stands in where it does not cover the call)
         native = _native_node(x)
         outs = () if native is None else native.recurrence_apply(x, log_decay, s_init, ops._debug_flags, ops._status_ptr(x))
-        return tuple(outs) or super().apply(x, log_decay, s_init)
+        return tuple(outs) or _GatedLinearRecurrence.apply(x, log_decay, s_init)
 
+
+class _LayerNorm(Function):
     @staticmethod
-    def forward(ctx: Any, x, log_decay, s_init=None):
-        out, s_final, states = recurrence.recurrence_fwd(x, log_decay, s_init, any(ctx.needs_input_grad[:3]))
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, log_decay, states)
-        return out, s_final
+    def forward(ctx: Any, x, weight=None, bias=None, eps: float = 1e-5):
+        out, _, stats = layer_norm.layer_norm_fwd(x, weight, bias, eps, None, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, stats)
+        return out
 
     @staticmethod
     @once_differentiable
-    def backward(ctx: Any, grad_output, grad_s_final):
-        x, log_decay, states = ctx.saved_tensors
-        if grad_output is None and grad_s_final is None:
-            return None, None, None
-        needs = tuple(ctx.needs_input_grad) + (False,) * (3 - len(ctx.needs_input_grad))
-        return tuple(recurrence.recurrence_bwd(grad_output, x, log_decay, states, grad_s_final, needs)[:len(ctx.needs_input_grad)])
+    def backward(ctx: Any, grad_output):
+        needs = (tuple(ctx.needs_input_grad) + (False,) * 3)[:3]
+        grads = layer_norm.layer_norm_bwd(grad_output, *ctx.saved_tensors, None, needs)
+        return (*grads, None)[:len(ctx.needs_input_grad)]
 
 
-class LayerNorm(Function):
+class LayerNorm(_LayerNorm):
     """Layer norm over the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``.
 
     ``LayerNorm.apply(x, weight=None, bias=None, eps=1e-5)`` for x ``[..., D]`` of any rank and strides (bf16, fp16 or fp32, D
@@ -313,37 +334,10 @@ class LayerNorm(Function):
     def apply(cls, x, weight=None, bias=None, eps: float = 1e-5):
         native = _native_node(x)
         outs = () if native is None else native.layer_norm_apply(x, None, weight, bias, eps)
-        return outs[0] if outs else super().apply(x, weight, bias, eps)
-
-    @staticmethod
-    def forward(ctx: Any, x, weight=None, bias=None, eps: float = 1e-5):
-        out, _, stats = layer_norm.layer_norm_fwd(x, weight, bias, eps, None, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, bias, stats)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad_output):
-        needs = (tuple(ctx.needs_input_grad) + (False,) * 3)[:3]
-        grads = layer_norm.layer_norm_bwd(grad_output, *ctx.saved_tensors, None, needs)
-        return (*grads, None)[:len(ctx.needs_input_grad)]
+        return outs[0] if outs else _LayerNorm.apply(x, weight, bias, eps)
 
 
-class AddLayerNorm(Function):
-    """Addition of a residual and layer norm in one pass: ``sum = x + residual`` (rounded to their type),
-    ``out = LayerNorm(sum)``.
-
-    ``out, sum = AddLayerNorm.apply(x, residual, weight=None, bias=None, eps=1e-5)``, shapes and types as for ``LayerNorm``.
-    ``sum`` is the residual of the next block, and its gradient joins that of ``out`` in one pass backward: x and the
-    residual get the same gradient. The reference has no counterpart.
-    """
-
-    @classmethod
-    def apply(cls, x, residual, weight=None, bias=None, eps: float = 1e-5):
-        native = _native_node(x)
-        outs = () if native is None or residual is None else native.layer_norm_apply(x, residual, weight, bias, eps)
-        return tuple(outs) or super().apply(x, residual, weight, bias, eps)
-
+class _AddLayerNorm(Function):
     @staticmethod
     def forward(ctx: Any, x, residual, weight=None, bias=None, eps: float = 1e-5):
         out, total, stats = layer_norm.layer_norm_fwd(x, weight, bias, eps, residual, any(ctx.needs_input_grad[:4]))
@@ -360,3 +354,19 @@ class AddLayerNorm(Function):
         needs = (tuple(ctx.needs_input_grad) + (False,) * 4)[:4]
         dx, dw, db = layer_norm.layer_norm_bwd(grad_output, *ctx.saved_tensors, grad_sum, (needs[0] or needs[1], *needs[2:]))
         return (dx, dx, dw, db, None)[:count]
+
+
+class AddLayerNorm(_AddLayerNorm):
+    """Addition of a residual and layer norm in one pass: ``sum = x + residual`` (rounded to their type),
+    ``out = LayerNorm(sum)``.
+
+    ``out, sum = AddLayerNorm.apply(x, residual, weight=None, bias=None, eps=1e-5)``, shapes and types as for ``LayerNorm``.
+    ``sum`` is the residual of the next block, and its gradient joins that of ``out`` in one pass backward: x and the
+    residual get the same gradient. The reference has no counterpart.
+    """
+
+    @classmethod
+    def apply(cls, x, residual, weight=None, bias=None, eps: float = 1e-5):
+        native = _native_node(x)
+        outs = () if native is None or residual is None else native.layer_norm_apply(x, residual, weight, bias, eps)
+        return tuple(outs) or _AddLayerNorm.apply(x, residual, weight, bias, eps)

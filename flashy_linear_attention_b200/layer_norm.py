@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import FlaLayerNormArgs
-from .ops import _desc
+from .ops import _desc, _stream
 from .recurrence import _DTYPES
 
 MAX_DIM = 32768  # columns of a row
@@ -88,7 +88,7 @@ def _args(x: torch.Tensor, weight, bias, eps: float) -> FlaLayerNormArgs:
 
 def _call(name: str, a: FlaLayerNormArgs, device: torch.device) -> None:
     with torch.cuda.device(device):
-        a.stream = torch.cuda.current_stream(device).cuda_stream
+        a.stream = _stream(device)
         rc = getattr(_lib.load(), name)(ctypes.byref(a))
     if rc != 0:
         raise RuntimeError(f"flashlinear: {name} returned {rc}: {_lib.strerror(rc)}")

@@ -210,6 +210,12 @@ def _dtype_code(t: torch.Tensor) -> int:
     return _lib.FLA_DTYPE_F16 if t.dtype == torch.float16 else _lib.FLA_DTYPE_BF16
 
 
+def _stream(device: torch.device) -> int:
+    """Address of the current stream. (Inside torch.compile, which traces the Python route of a call piece by piece,
+    torch.cuda.current_stream() is an object that does not have it.)"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _desc(t: Optional[torch.Tensor]) -> FlaTensor:
     if t is None:
         return FlaTensor(None, 0, 0, 0)

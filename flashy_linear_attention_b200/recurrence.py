@@ -12,7 +12,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import FlaRecurrenceArgs
-from .ops import _desc
+from .ops import _desc, _stream
 
 _DTYPES = {
     torch.bfloat16: _lib.FLA_DTYPE_BF16,
@@ -77,7 +77,7 @@ def _args(x: torch.Tensor, g: torch.Tensor) -> FlaRecurrenceArgs:
 
 def _call(name: str, a: FlaRecurrenceArgs, device: torch.device) -> None:
     with torch.cuda.device(device):
-        a.stream = torch.cuda.current_stream(device).cuda_stream
+        a.stream = _stream(device)
         a.status, a.debug_flags = ops._status_word(device).data_ptr(), ops._debug_flags
         rc = getattr(_lib.load(), name)(ctypes.byref(a))
     if rc != 0:

@@ -1,0 +1,25 @@
+"""The Functions beside an attention without a GPU: what they refuse, also inside torch.compile."""
+import warnings
+
+import pytest
+import torch
+
+
+def calls():
+    from flashy_linear_attention_b200 import AddLayerNorm, GatedLinearRecurrence, LayerNorm
+
+    return [lambda t: LayerNorm.apply(t), lambda t: LayerNorm.apply(t, t[0, 0, 0], None, 1e-3), lambda t: AddLayerNorm.apply(t, t),
+            lambda t: GatedLinearRecurrence.apply(t, t), lambda t: GatedLinearRecurrence.apply(t, t, t[:, :, 0])]
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_compiled_call_is_refused_like_any_other(which, grad):
+    call, x = calls()[which], torch.zeros(1, 1, 4, 8, requires_grad=grad)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        call(x)
+    torch._dynamo.reset()
+    with warnings.catch_warnings(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        warnings.simplefilter("ignore")
+        torch.compile(call, backend="eager")(x)
+    torch._dynamo.reset()
