@@ -66,7 +66,7 @@ def _first_use(device: torch.device, status: torch.Tensor) -> None:
     if torch.cuda.is_current_stream_capturing():
         return
     lib = _lib.load()
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _stream(device)
     with torch.cuda.device(device):
         for d in (64, 128):
             x = torch.ones(1, 160, 128, d, dtype=torch.bfloat16, device=device)  # a CTA on every SM
@@ -152,7 +152,7 @@ def _rows_call(name: str, src: torch.Tensor, dst: torch.Tensor, rows: int, d: in
     lib = _lib.load()
     with torch.cuda.device(src.device):
         rc = getattr(lib, name)(src.data_ptr(), dst.data_ptr(), rows, d, dpad,
-                                torch.cuda.current_stream(src.device).cuda_stream)
+                                _stream(src.device))
     if rc != 0:
         raise RuntimeError(f"flashlinear: {name} returned {rc}: {_lib.strerror(rc)}")
 
@@ -236,7 +236,7 @@ def _call(pass_id: int, args: FlaArgs, device: torch.device, which: int = 0,
     caller hands in `workspace`; the scratch tensor (or None) is returned."""
     lib = _lib.load()
     with torch.cuda.device(device):
-        args.stream = torch.cuda.current_stream(device).cuda_stream
+        args.stream = _stream(device)
         args.status = _status_word(device).data_ptr()
         args.debug_flags = _debug_flags
         need = lib.fla_sm100_workspace_bytes(ctypes.byref(args), 0 if pass_id == 3 else pass_id)
@@ -485,7 +485,7 @@ def causal_dot_product_bwd(
 def _norm_args(ref: torch.Tensor, dk: int, dv: int) -> FlaArgs:
     a = FlaArgs()
     a.batch, a.heads, a.seqlen, a.dk, a.dv = ref.shape[0], ref.shape[1], ref.shape[2], dk, dv
-    a.stream = torch.cuda.current_stream(ref.device).cuda_stream
+    a.stream = _stream(ref.device)
     a.status = _status_word(ref.device).data_ptr()
     return a
 
@@ -605,7 +605,7 @@ def normalized_bwd(dnum, dden, q, k, v, s_last):
     if not all(_addressable(t) for t in outs):
         return None
     with torch.cuda.device(q.device):
-        a.stream = torch.cuda.current_stream(q.device).cuda_stream
+        a.stream = _stream(q.device)
         a.status = _status_word(q.device).data_ptr()
         a.q, a.k, a.v, a.d_o = _desc(q), _desc(k), _desc(v), _desc(dnum)
         a.d_q, a.d_k, a.d_v = (_desc(t) for t in outs)
@@ -667,7 +667,7 @@ def _taylor_call(name: str, xq, xk, v, **tensors) -> None:
     for key, t in dict(tensors, q=_kernel_view(xq), k=_kernel_view(xk), v=_kernel_view(v)).items():
         setattr(args, key, _desc(t))
     with torch.cuda.device(xq.device):
-        args.stream = torch.cuda.current_stream(xq.device).cuda_stream
+        args.stream = _stream(xq.device)
         args.status = _status_word(xq.device).data_ptr()
         args.debug_flags = _debug_flags
         rc = getattr(_lib.load(), name)(ctypes.byref(args))
@@ -757,7 +757,7 @@ def taylor_features(x: torch.Tensor) -> torch.Tensor:
     buf = torch.empty(x.shape[:-1] + (fp.value,), dtype=x.dtype, device=x.device)
     with torch.cuda.device(x.device):
         rc = lib.fla_sm100_taylor_features(xc.data_ptr(), buf.data_ptr(), xc.numel() // d, d,
-                                           torch.cuda.current_stream(x.device).cuda_stream)
+                                           _stream(x.device))
     _norm_check(rc, "fla_sm100_taylor_features")
     return buf[..., :f.value]
 
@@ -783,7 +783,7 @@ def taylor_features_bwd(dphi: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     dx = torch.empty_like(xc)
     with torch.cuda.device(x.device):
         rc = lib.fla_sm100_taylor_features_bwd(dphi.data_ptr(), xc.data_ptr(), dx.data_ptr(), rows, d,
-                                               torch.cuda.current_stream(x.device).cuda_stream)
+                                               _stream(x.device))
     _norm_check(rc, "fla_sm100_taylor_features_bwd")
     return dx
 

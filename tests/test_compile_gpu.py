@@ -5,7 +5,7 @@ import warnings
 import pytest
 import torch
 
-from test_block_gpu import DEV, functions
+from test_block_gpu import DEV, block, functions, inputs, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -58,6 +58,19 @@ def test_single_functions(native, backend):
             assert all(torch.equal(a, b) for a, b in zip(step(compiled, leaves), step(call, leaves))), name
         with torch.no_grad():
             assert all(torch.equal(a, b) for a, b in zip(compiled(*leaves), call(*leaves))), name
+
+
+def test_a_block(native):
+    tensors = inputs(70)
+    w = {name: t.to(torch.bfloat16) for name, t in weights().items()}
+    names = list(w)
+
+    def call(branch, residual, *ws):
+        return block(dict(zip(names, ws)), branch, residual)[:2]
+
+    leaves = (*tensors[:2], *w.values())
+    compiled = torch.compile(call, backend="eager")
+    assert all(torch.equal(a, b) for a, b in zip(step(compiled, leaves), step(call, leaves)))
 
 
 def test_refusals(native):
