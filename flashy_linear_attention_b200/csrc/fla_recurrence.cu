@@ -73,9 +73,12 @@ struct RunMap {
   float2 hi, lo, b;
 };
 
+// A factor that underflows leaves nothing of a state, however large, but an infinity stays one until a gate of minus infinity (and
+// without `lo`, which would make a NaN of two opposite ones).
+constexpr float kLeastDecay = 1.17549435e-38f, kMostDecay = 3.40282347e38f;
 __device__ __forceinline__ float apply_map(float c, float hi, float lo, float b) {
-  const float low = fabsf(c) <= 3.4e38f ? fmaf(lo, c, b) : b;  // (two opposite infinities would make a NaN)
-  return hi < 0.f ? b : fmaf(hi, c, low);
+  const float finite = fmaf(hi, c, fmaf(lo, c, b)), infinite = fmaf(hi < kLeastDecay ? kLeastDecay : hi, c, b);
+  return hi < 0.f ? b : fabsf(c) <= kMostDecay ? finite : infinite;
 }
 __device__ __forceinline__ float2 apply_map(float2 c, const RunMap& m) {
   return make_float2(apply_map(c.x, m.hi.x, m.lo.x, m.b.x), apply_map(c.y, m.hi.y, m.lo.y, m.b.y));
@@ -102,12 +105,6 @@ __device__ __forceinline__ void split_exp(float s, float* hi, float* lo) {
   *hi = near ? 1.f + e : s == -INFINITY ? -1.f : fast_exp2(s * kLog2e);
   *lo = near ? e - (*hi - 1.f) : 0.f;
 }
-// The factor of a run is kept inside the normal numbers: below, what it adds is less than 2^-126 of the state, but an
-// infinity stays one until a gate of minus infinity, as it does token by token; above, a state of zero stays zero.
-constexpr float kLeastDecay = 1.17549435e-38f, kMostDecay = 3.40282347e38f;
-__device__ __forceinline__ float normal(float hi) {
-  return fabsf(hi) < kLeastDecay ? kLeastDecay : hi > kMostDecay ? kMostDecay : hi;
-}
 __device__ __forceinline__ RunMap token_map(float2 g, float2 b) {
   RunMap m;
   m.b = b;
@@ -115,9 +112,11 @@ __device__ __forceinline__ RunMap token_map(float2 g, float2 b) {
   split_exp(g.y, &m.hi.y, &m.lo.y);
   return m;
 }
+// (a run's factor past the largest number leaves a state of zero zero)
+__device__ __forceinline__ float at_most(float hi) { return hi > kMostDecay ? kMostDecay : hi; }
 __device__ __forceinline__ RunMap run_map(float2 sum, float2 b) {
   RunMap m = token_map(sum, b);
-  m.hi = make_float2(normal(m.hi.x), normal(m.hi.y));
+  m.hi = make_float2(at_most(m.hi.x), at_most(m.hi.y));
   return m;
 }
 

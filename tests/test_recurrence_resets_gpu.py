@@ -129,3 +129,27 @@ def test_no_bit_of_a_channel_depends_on_another(kind, N):
             spoiled, up = x.clone(), dy.clone()
             spoiled[..., at, 3], up[..., at, 3] = value, value
             others(run(spoiled, other, s, up, ds), clean, 3, f"row and gate {at} {value}")
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("drop", [-1e4, "lowest"])
+def test_a_gate_whose_decay_underflows_leaves_nothing_of_the_largest_state(kind, drop):
+    """Rows of their type's lowest value, as in masked places, before a gate so low that its decay is zero: also where the gate is the
+    only low one of its run and the state comes from the run before."""
+    N, D, dtype, gate = 400, *kind
+    for at in (17, 48, 208, 256):
+        x, g, s, dy, ds = make(N, D, dtype, gate)
+        g[:, :, at] = torch.finfo(gate).min if drop == "lowest" else drop
+        x[:, :, at - 1] = 0
+        clean = run(x, g, s, dy, ds)
+        x[:, :, at - 1] = torch.finfo(dtype).min
+        got = run(x, g, s, dy, ds)
+        same(got["out"][:, :, at:], clean["out"][:, :, at:], "out")
+        same(got["s_final"], clean["s_final"], "s_final")
+        x[:, :, at - 1] = 0
+        dy[:, :, at] = 0
+        clean = run(x, g, s, dy, ds)
+        dy[:, :, at] = torch.finfo(dtype).min
+        got = run(x, g, s, dy, ds)
+        same(got["dx"][:, :, :at], clean["dx"][:, :, :at], "dx")
+        same(got["ds"], clean["ds"], "ds")
