@@ -1234,8 +1234,9 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward, int sm_count) {
                 return reinterpret_cast<uintptr_t>(t.ptr) % (2 * size) == 0 && (p.n == 1 || t.sn % 2 == 0) &&
                        (p.heads == 1 || t.sh % 2 == 0) && (plan.batch == 1 || t.sb % 2 == 0);
               });
+  const long long columns = p.c;  // (up to 2^30: what is formed from it passes 32 bits)
   auto rows_on = [&](int bytes) {
-    return p.c * sizes[0] % bytes == 0 && p.c * sizes[1] % bytes == 0 && every([&](const RecurrenceTensor& t, int size) {
+    return columns * sizes[0] % bytes == 0 && columns * sizes[1] % bytes == 0 && every([&](const RecurrenceTensor& t, int size) {
              return reinterpret_cast<uintptr_t>(t.ptr) % bytes == 0 && (p.n == 1 || t.sn * size % bytes == 0) &&
                     (p.heads == 1 || t.sh * size % bytes == 0) && (plan.batch == 1 || t.sb * size % bytes == 0);
            });
@@ -1250,9 +1251,9 @@ Plan make_plan(const FlaRecurrenceArgs* a, bool backward, int sm_count) {
   // leave places on the SMs empty. Microseconds forward + backward with tiles of 64 and 32: 8 x 128 channels, 65536 tokens, bf16
   // 215 + 306 / 128 + 214, fp32 403 + 531 / 204 + 303; 4 x 256 channels, 8192 tokens 38 + 44 / 23 + 34; but 32 x 128 channels,
   // 2048 tokens 19 + 27 / 19 + 32, and 128 x 64 channels, 4096 tokens 48 + 82 / 52 + 89.
-  const long long tiles64 = (p.c + 63LL) / 64 * p.heads * plan.batch;
-  plan.lpr = (p.c + 31) / 32 * 32 * 10 < (p.c + 63) / 64 * 64 * 9 || tiles64 * fla::kRecMaxCluster <= 2 * sm_count ? 16 : 32;
-  p.tiles = (p.c + 2 * plan.lpr - 1) / (2 * plan.lpr);
+  const long long tiles64 = (columns + 63) / 64 * p.heads * plan.batch;
+  plan.lpr = (columns + 31) / 32 * 32 * 10 < (columns + 63) / 64 * 64 * 9 || tiles64 * fla::kRecMaxCluster <= 2 * sm_count ? 16 : 32;
+  p.tiles = static_cast<int>((columns + 2 * plan.lpr - 1) / (2 * plan.lpr));
   p.tiles_all = static_cast<long long>(p.tiles) * p.heads * plan.batch;
   return plan;
 }
