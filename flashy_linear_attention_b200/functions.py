@@ -367,6 +367,8 @@ class AddLayerNorm(_AddLayerNorm):
 
     @classmethod
     def apply(cls, x, residual, weight=None, bias=None, eps: float = 1e-5):
+        if residual is None:
+            raise ValueError("flashlinear: AddLayerNorm needs a residual (LayerNorm is the norm without one)")
         native = _native_node(x)
-        outs = () if native is None or residual is None else native.layer_norm_apply(x, residual, weight, bias, eps)
+        outs = () if native is None else native.layer_norm_apply(x, residual, weight, bias, eps)
         return tuple(outs) or _AddLayerNorm.apply(x, residual, weight, bias, eps)

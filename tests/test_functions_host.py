@@ -4,6 +4,8 @@ import warnings
 import pytest
 import torch
 
+from test_recurrence_host import fake
+
 
 def calls():
     from flashy_linear_attention_b200 import AddLayerNorm, GatedLinearRecurrence, LayerNorm
@@ -23,3 +25,13 @@ def test_a_compiled_call_is_refused_like_any_other(which, grad):
         warnings.simplefilter("ignore")
         torch.compile(call, backend="eager")(x)
     torch._dynamo.reset()
+
+
+def test_a_residual_that_is_not_there_is_refused():
+    from flashy_linear_attention_b200 import AddLayerNorm
+
+    for x in (torch.zeros(4, 8), fake(4, 8), fake(4, 8).requires_grad_(True)):
+        with pytest.raises(ValueError, match="residual"):
+            AddLayerNorm.apply(x, None)
+        with pytest.raises(ValueError, match="residual"):
+            AddLayerNorm.apply(x, None, fake(8), fake(8), 1e-3)
