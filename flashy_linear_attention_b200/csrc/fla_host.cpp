@@ -418,9 +418,8 @@ bool recurrence_covered(const Tensor& x, const Tensor& g) {
   if (!recurrence_rows(x) || !recurrence_rows(g) || x.sizes() != g.sizes() || x.device() != g.device() || x.numel() == 0)
     return false;
   if (float_type(x) < 0 || (float_type(g) != float_type(x) && float_type(g) != FLA_DTYPE_F32)) return false;
-  for (int d = 0; d < 4; ++d)
-    if (x.size(d) > INT32_MAX) return false;
-  return true;
+  constexpr int64_t kMost = 1 << 30;
+  return x.size(0) <= kMost && x.size(1) <= kMost && x.size(0) * x.size(1) <= kMost && x.size(2) <= kMost && x.size(3) <= kMost;
 }
 bool channel_state(const OptTensor& s, const Tensor& x) {
   return !s.has_value() || (s->is_cuda() && s->device() == x.device() && s->scalar_type() == at::kFloat && s->dim() == 3 &&

@@ -20,6 +20,8 @@ _DTYPES = {
     torch.float32: _lib.FLA_DTYPE_F32,
 }
 
+MAX_SIZE = 2**30  # tokens, channels of a head, heads of all sequences
+
 
 def _check_state(s: Optional[torch.Tensor], name: str, x: torch.Tensor) -> None:
     if s is None:
@@ -49,6 +51,10 @@ def check_inputs(x: torch.Tensor, log_decay: torch.Tensor, s_init: Optional[torc
     if log_decay.shape != x.shape:
         raise ValueError(f"flashlinear: x and log_decay must have the same shape, got {tuple(x.shape)} and "
                          f"{tuple(log_decay.shape)} (expand a gate that channels, heads or tokens share)")
+    B, H, N, D = x.shape
+    if x.numel() and max(B * H, N, D) > MAX_SIZE:
+        raise ValueError(f"flashlinear: the recurrence takes up to 2^30 tokens, 2^30 channels a head and 2^30 heads of all "
+                         f"sequences, got {tuple(x.shape)}")
     _check_state(s_init, "s_init", x)
 
 

@@ -35,3 +35,18 @@ def test_a_residual_that_is_not_there_is_refused():
             AddLayerNorm.apply(x, None)
         with pytest.raises(ValueError, match="residual"):
             AddLayerNorm.apply(x, None, fake(8), fake(8), 1e-3)
+
+
+def test_sizes_past_the_recurrence_are_refused():
+    """Sizes of 2^32 and more would otherwise lose their upper bits on the way to the library."""
+    from flashy_linear_attention_b200 import recurrence
+
+    for shape in ((1, 1, 2**30, 1), (1, 1, 1, 2**30), (2**15, 2**15, 1, 1)):
+        t = fake(1).expand(shape)
+        recurrence.check_inputs(t, t)
+    for shape in ((1, 1, 2**30 + 1, 1), (1, 1, 2**32 + 5, 1), (1, 1, 1, 2**32 + 5), (2**32 + 5, 1, 1, 1), (1, 2**30 + 1, 1, 1), (2**16, 2**16, 1, 1)):
+        t = fake(1).expand(shape)
+        with pytest.raises(ValueError, match="2.30"):
+            recurrence.check_inputs(t, t)
+    empty = fake(0).reshape(2**32, 0, 1, 1)
+    recurrence.check_inputs(empty, empty)
