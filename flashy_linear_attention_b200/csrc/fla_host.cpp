@@ -569,7 +569,8 @@ std::optional<std::array<OptTensor, 3>> layer_norm_backward(const Tensor& dy, co
                                                             const Tensor& stats, const OptTensor& ds, bool need_x, bool need_w,
                                                             bool need_b) {
   if (!norm_covered(x, w, b) || !norm_rows(dy, x) || (ds.has_value() && !norm_rows(*ds, x)) || !stats.is_cuda() ||
-      stats.scalar_type() != at::kFloat || !stats.is_contiguous() || !(need_x || need_w || need_b))
+      stats.device() != x.device() || stats.scalar_type() != at::kFloat || !stats.is_contiguous() ||
+      stats.numel() != 2 * (x.numel() / x.size(-1)) || !(need_x || need_w || need_b))
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
   FlaLayerNormArgs a = norm_args(x, w, b, 0.0);

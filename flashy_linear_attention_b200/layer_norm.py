@@ -160,6 +160,9 @@ def layer_norm_bwd(
         return dx, *(None if t is None else t.zero_() for t in (dw, db))
     if not any(needs):
         return None, None, None
+    if (not stats.is_cuda or stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous()
+            or stats.numel() != 2 * (x.numel() // x.shape[-1])):
+        raise ValueError("flashlinear: the backward needs the statistics of a forward over these rows with keep_stats=True")
     for g in (grad_out, grad_sum):
         if g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device):
             raise ValueError("flashlinear: gradients of the outputs must have their shape, type and device")

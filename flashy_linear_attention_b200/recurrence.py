@@ -157,6 +157,10 @@ def recurrence_bwd(
         return dx, dg, ds
     if not any(needs):
         return None, None, None
+    if states is None:
+        raise ValueError("flashlinear: the backward needs the states of a forward with keep_states=True")
+    if not states.is_cuda or states.device != x.device or not states.is_contiguous():
+        raise ValueError("flashlinear: the states of the forward must be contiguous and on the device of x")
     a = _args(x, g)
     if grad_out is not None:
         if grad_out.shape != x.shape or grad_out.dtype != x.dtype or grad_out.device != x.device:
@@ -165,8 +169,6 @@ def recurrence_bwd(
     a.d_o, a.d_x, a.d_g = _desc(grad_out), _desc(dx), _desc(dg)
     a.r_init = None if r_init is None else r_init.data_ptr()
     a.r_final = None if ds is None else ds.data_ptr()
-    if states is None:
-        raise ValueError("flashlinear: the backward needs the states of a forward with keep_states=True")
-    a.states, a.states_bytes = states.data_ptr(), states.numel()
+    a.states, a.states_bytes = states.data_ptr(), states.numel() * states.element_size()
     _call("fla_sm100_recurrence_bwd", a, x.device)
     return dx, dg, ds

@@ -50,3 +50,18 @@ def test_sizes_past_the_recurrence_are_refused():
             recurrence.check_inputs(t, t)
     empty = fake(0).reshape(2**32, 0, 1, 1)
     recurrence.check_inputs(empty, empty)
+
+
+def test_what_a_forward_kept_is_checked_before_its_address_is_used(monkeypatch):
+    """It may come back from a hook of autograd's: from the host, shortened, of another type."""
+    from flashy_linear_attention_b200 import _lib, layer_norm, recurrence
+
+    monkeypatch.setattr(_lib, "host", lambda: None)
+    x = fake(2, 3, 40, 8)
+    for states in (None, torch.zeros(4096, dtype=torch.uint8), fake(4096, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="states"):
+            recurrence.recurrence_bwd(x, x, x, states)
+    rows = fake(5, 8)
+    for stats in (torch.zeros(5, 2), fake(4, 2), fake(5, 2, dtype=torch.float64), fake(2, 5).t()):
+        with pytest.raises(ValueError, match="statistics"):
+            layer_norm.layer_norm_bwd(rows, rows, None, None, stats)
