@@ -477,7 +477,7 @@ std::optional<std::array<OptTensor, 3>> recurrence_backward(const OptTensor& dy,
   Tensor rows;
   if (dy.has_value()) {
     if (dy->sizes() != x.sizes() || dy->scalar_type() != x.scalar_type() || dy->device() != x.device()) return std::nullopt;
-    rows = recurrence_rows(*dy) ? *dy : dy->contiguous();
+    rows = recurrence_rows(*dy) ? *dy : dy->resolve_neg().contiguous();
     if (!recurrence_rows(rows)) return std::nullopt;
     a.d_o = desc(rows);
   }
@@ -641,7 +641,7 @@ struct RecurrenceNode : torch::autograd::Function<RecurrenceNode> {
     const int64_t wants = ctx->saved_data["wants"].toInt();
     {
       const at::AutoGradMode off(false);
-      const Tensor ds = grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : Tensor();
+      const Tensor ds = grads[1].defined() ? grads[1].resolve_neg().to(at::kFloat).contiguous() : Tensor();
       const auto r = recurrence_backward(or_null(grads[0]), saved[0], saved[1], saved[2], or_null(ds), wants & 1, wants & 2, wants & 4,
                                          static_cast<unsigned>(ctx->saved_data["flags"].toInt()),
                                          static_cast<uintptr_t>(ctx->saved_data["status"].toInt()));
@@ -681,7 +681,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     const int64_t wants = ctx->saved_data["wants"].toInt();
     {
       const at::AutoGradMode off(false);
-      auto rows = [&](const Tensor& t) { return !t.defined() || norm_rows(t, saved[0]) ? t : t.contiguous(); };
+      auto rows = [&](const Tensor& t) { return !t.defined() || norm_rows(t, saved[0]) ? t : t.resolve_neg().contiguous(); };
       const auto r = layer_norm_backward(rows(grads[0]), saved[0], or_null(saved[1]), or_null(saved[2]), saved[3], or_null(rows(ds)),
                                          wants & 1, wants & 2, wants & 4);
       if (!r.has_value()) throw std::runtime_error("flashlinear: the gradients of the layer norm's outputs do not fit them");
