@@ -499,7 +499,8 @@ bool norm_rows(const Tensor& t, const Tensor& x) {
 }
 bool norm_weights(const OptTensor& w, const Tensor& x) {
   if (!w.has_value()) return true;
-  if (!w->is_cuda() || w->device() != x.device() || !w->is_contiguous() || w->is_neg() || w->size(-1) != x.size(-1)) return false;
+  if (!w->is_cuda() || w->device() != x.device() || !w->is_contiguous() || w->is_neg()) return false;
+  if (w->dim() < 1 || w->size(-1) != x.size(-1)) return false;
   if (w->dim() != 1 && !(w->dim() == 2 && x.dim() == 4 && w->size(0) == x.size(1))) return false;
   return float_type(*w) == float_type(x) || float_type(*w) == FLA_DTYPE_F32;
 }

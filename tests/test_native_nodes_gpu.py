@@ -35,3 +35,13 @@ def test_inputs_with_a_lazy_sign(native):
         want = call(*inputs)
         got = call(*(torch._neg_view(-t) for t in inputs))
         assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
+def test_weights_of_no_dimension_are_refused_like_any_of_a_wrong_shape(native):
+    fla = functions()
+    x, one = torch.randn(5, 8, device=DEV), torch.ones((), device=DEV)
+    for w, b in ((one, None), (None, one), (torch.ones(8, device=DEV), one)):
+        with pytest.raises(ValueError, match="must have shape"):
+            fla.LayerNorm.apply(x, w, b)
+        with pytest.raises(ValueError, match="must have shape"):
+            fla.AddLayerNorm.apply(x, x, w, b)
