@@ -294,8 +294,10 @@ class GatedLinearRecurrence(_GatedLinearRecurrence):
     @classmethod
     def apply(cls, x, log_decay, s_init=None):
         if torch.is_autocast_enabled("cuda"):
-            x = x.to(torch.bfloat16)
-            if log_decay.dtype != torch.float32:
+            # (of the types that autocast casts; others are refused as they are without it)
+            if x.dtype in (torch.float16, torch.float32):
+                x = x.to(torch.bfloat16)
+            if log_decay.dtype == torch.float16:
                 log_decay = log_decay.to(torch.bfloat16)
         # (a native autograd node, for which the Python Function above stands in where it does not cover the call)
         native = _native_node(x)

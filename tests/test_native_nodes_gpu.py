@@ -45,3 +45,16 @@ def test_weights_of_no_dimension_are_refused_like_any_of_a_wrong_shape(native):
             fla.LayerNorm.apply(x, w, b)
         with pytest.raises(ValueError, match="must have shape"):
             fla.AddLayerNorm.apply(x, x, w, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int32, torch.bool])
+def test_autocast_makes_no_call_right_that_is_refused_without_it(native, dtype):
+    fla = functions()
+    x, g = torch.ones(1, 2, 5, 8, device=DEV), torch.zeros(1, 2, 5, 8, device=DEV)
+    for autocast in (False, True):
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            for args in ((x.to(dtype), g), (x, g.to(dtype))):
+                with pytest.raises(TypeError, match="flashlinear"):
+                    fla.GatedLinearRecurrence.apply(*args)
+            with pytest.raises(TypeError, match="flashlinear"):
+                fla.LayerNorm.apply(x.to(dtype))
