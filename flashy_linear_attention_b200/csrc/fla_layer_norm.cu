@@ -15,7 +15,7 @@
 //
 // Measured (B200, of the 6.45 TB/s of a copy), bf16: 32768 rows of 4096 forward 97 us (86 %), backward 149 (84 %), with a
 // residual 194 (86 %) and 173 (96 %); 1048576 rows of 128 101 (83 %) and 150 (83 %); 524288 rows of 64 in fp16 26 us
-// (79 %). Rows that are no multiple of 16 bytes go element by element: 142848 rows of 83 in fp32 34 (43 %) and 52 (42 %).
+// (79 %). Rows that are no multiple of 16 bytes go element by element: 142848 rows of 83 in fp32 33 (45 %) and 51 (43 %).
 #include <algorithm>
 #include <type_traits>
 

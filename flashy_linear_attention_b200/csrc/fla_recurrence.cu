@@ -20,16 +20,18 @@
 // Four ways, by what rows allow: short sequences alone in a warp; rows on 16-byte or 4-byte boundaries through tiles in
 // shared memory; 16-bit rows of odd widths by direct loads. Measured (B200, of the 6.45 TB/s of a copy): 4 x 32 heads,
 // 8192 x 128 in bf16 forward 146 us (85 %), backward 236 (88 %), a tenth more once the GPU draws its full power; 65536 tokens of
-// 8 x 128 channels with fp32 gates 151 (55 %) and 264 (55 %); 3 x 24 heads, 1984 x 83 in fp32 71 (31 %) and 84 (44 %): the 4-byte
-// copies. Few channels are bound by the time of a step (1.2 us, 2 in a cluster of eight), whatever the rows hold: 65536 tokens of
-// 64 channels 68 and 132 us.
+// 8 x 128 channels with fp32 gates 152 (55 %) and 270 (54 %); 3 x 24 heads, 1984 x 83 in fp32 74 (30 %) and 88 (42 %): the 4-byte
+// copies; 4 x 32 heads, 8192 x 83 in bf16 299 (27 %) and 580 (23 %): direct loads of single elements, whose registers spill. Few
+// channels are bound by the time of a step (1.2 us, 2 in a cluster of eight), whatever the rows hold: 65536 tokens of
+// 64 channels 68 and 127 us.
 //
 // Accuracy. Channels with a memory of ten thousand tokens multiply the state by exp(-1e-4) as often. That
 // factor rounded to 32 bits is off by up to 3e-8, every time in the same direction. The state is therefore multiplied
-// once a run, by exp(sum of g) held as two floats; the decays of single tokens only act within a run.
+// once a run, by exp(sum of g) held as two floats; the decays of single tokens only act within a run. 16-bit rows take those from the
+// fast exponential (off by 2^-22), which is all that their fp32 results (states, and gradients of fp32 gates) are off by beyond roundings.
 //
-// A gate of minus infinity (a document starts) drops the state whatever it holds, infinities and NaN included, and
-// nothing flows back past it.
+// A gate of minus infinity (a document starts) drops the state whatever it holds, infinities and NaN included, whatever gates stand
+// beside it, and nothing flows back past it.
 #include <cooperative_groups.h>
 
 #include <algorithm>

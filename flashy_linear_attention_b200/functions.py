@@ -281,7 +281,9 @@ class GatedLinearRecurrence(_GatedLinearRecurrence):
     (bf16, fp16 or fp32; log_decay of the same type or fp32; any strides, broadcast by ``expand`` included) and fp32
     states ``[B, H, D]``, as ``LinearAttentionResumable`` has them: feeding ``s_final`` of one call as ``s_init`` of the
     next gives what one call over the concatenated tokens gives, for any number of tokens a call, one and none included.
-    ``out`` is h rounded to x's type; h itself is summed in fp32. All of x, log_decay and s_init are differentiable.
+    ``out`` is h rounded to x's type; h itself is summed in fp32. All of x, log_decay and s_init are differentiable. Sequences, channels
+    of a head and heads of a batch are up to 2^30. 16-bit rows take the decays inside 8 or 16 tokens from a fast exponential: fp32 results
+    of such calls (states, the gradient of an fp32 log_decay) are right to about 2^-18 of the sums behind them, those of fp32 rows to 2^-20.
 
     ``log_decay`` is usually at most 0 (a ``logsigmoid``, or minus a rate). -inf drops the state, whatever it holds: set
     it on the first token of each document of a packed row, and nothing passes between them, in either pass. 0, with x = 0,
@@ -327,7 +329,9 @@ class LayerNorm(_LayerNorm):
     up to 32768); weight and bias ``[D]``, or for x ``[B, H, N, D]`` also ``[H, D]``: an affine map of each head's own, which
     normalises an attention's unnormalised output head by head, the usual alternative to its denominator
     (``LinearAttentionNormalized``). They have x's type or fp32, and so have their gradients, which are summed in fp32 over
-    all rows in a fixed order and rounded once. Autocast changes nothing: the result has x's type.
+    all rows in a fixed order and rounded once. Autocast changes nothing: the result has x's type. Means and squares are summed in
+    fp32: a row whose squared differences pass its range (values beyond 1e18) is not normalised. ``[H, D]`` weights are for up to
+    65535 heads.
 
     The reference has no counterpart.
     """

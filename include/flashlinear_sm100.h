@@ -345,7 +345,8 @@ int fla_sm100_taylor_bwd(const FlaArgs* args);
 
 /* ---- gated linear recurrence ----
  * h_t = exp(g_t) h_(t-1) + x_t for every channel of [batch, heads, seqlen, dim] tensors, out_t = h_t. g_t = -inf drops the
- * state, whatever it holds (a document starts); g_t = 0 and x_t = 0 leave it as it is (a token to be passed over).
+ * state, whatever it holds (a document starts), NaN gates beside it included; g_t = 0 and x_t = 0 leave it as it is (a token
+ * to be passed over).
  * The reference has no counterpart. Tensors have any (batch, head, token) strides, zero for broadcast inputs and negative
  * ones included, and an innermost stride of 1; nothing has to be aligned beyond its element size; seqlen, dim and
  * batch * heads are up to 2^30. States are fp32
@@ -382,7 +383,8 @@ int fla_sm100_recurrence_bwd(const FlaRecurrenceArgs* args);
  * Rows of dim columns in [batch, heads, tokens, dim] tensors, any strides (zero included for inputs), innermost stride 1,
  * nothing aligned beyond its element size (faster where all rows are 16-byte aligned and dim is a multiple of 16 bytes).
  * dtype: of all rows; w_dtype: of weight, bias and their gradients, the same or fp32. weight and bias (each may be null)
- * are [dim], or with per_head [heads, dim], contiguous. dim up to 32768, rows up to 2^31 - 1.
+ * are [dim], or with per_head [heads, dim], contiguous. dim up to 32768, rows up to 2^31 - 1,
+ * heads with weights of their own up to 65535.
  * fwd: y = (s - mean) / sqrt(var + eps) * weight + bias with s = x, or, where residual is given, s = x + residual rounded to
  * dtype, which is written to sum. stats (optional, fp32 [2 * rows], 8-byte aligned, private to the library) is kept for:
  * bwd: x is the s of the forward, d_y the gradient of y, d_sum (optional) that of sum; writes d_x (the gradient of x and of the
