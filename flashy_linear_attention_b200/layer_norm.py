@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import FlaLayerNormArgs
-from .ops import _desc, _stream
+from .ops import _desc, untraced
 from .recurrence import _DTYPES
 
 MAX_DIM = 32768  # columns of a row
@@ -88,7 +88,7 @@ def _args(x: torch.Tensor, weight, bias, eps: float) -> FlaLayerNormArgs:
 
 def _call(name: str, a: FlaLayerNormArgs, device: torch.device) -> None:
     with torch.cuda.device(device):
-        a.stream = _stream(device)
+        a.stream = torch.cuda.current_stream(device).cuda_stream
         rc = getattr(_lib.load(), name)(ctypes.byref(a))
     if rc != 0:
         raise RuntimeError(f"flashlinear: {name} returned {rc}: {_lib.strerror(rc)}")
@@ -98,6 +98,7 @@ def _contiguous(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.resolve_neg().contiguous()
 
 
+@untraced
 def layer_norm_fwd(
     x: torch.Tensor,
     weight: Optional[torch.Tensor],
@@ -132,6 +133,7 @@ def layer_norm_fwd(
     return out, total, stats
 
 
+@untraced
 def layer_norm_bwd(
     grad_out: torch.Tensor,
     x: torch.Tensor,

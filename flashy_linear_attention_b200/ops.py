@@ -9,7 +9,9 @@ the denominator stays in PyTorch, as in the reference (README.md:22-30).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+import sys
 from typing import Optional, Tuple
 
 import torch
@@ -26,6 +28,31 @@ MAX_HEAD_DIM_QK_SMALLV = 512  # cap of q/k for LinearAttentionSmallVHD (273-dim 
 _status_words = {}
 # FLA_DEBUG_* bits passed with every call; FLA_DEBUG_FLAGS in the environment sets the initial value
 _debug_flags = int(os.environ.get("FLA_DEBUG_FLAGS", "0") or 0)
+
+
+_untraced_forms: dict = {}
+
+
+def _untraced_form(fn):
+    form = _untraced_forms.get(fn)
+    if form is None:
+        form = _untraced_forms[fn] = torch.compiler.disable(fn)
+    return form
+
+
+def untraced(fn):
+    """`fn` outside of what torch.compile traces, for what hands addresses of tensors to the library. Traced, a tensor is released at its
+    last use in Python, which is where its address is taken, and the next allocation gets its memory before the launch has
+    read it. (torch.compiler.disable() loads the compiler, which takes seconds, so that is left until it is there anyway. Where this
+    function is traced itself, is_compiling() is True to the tracer.)"""
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        if torch.compiler.is_compiling() or "torch._dynamo" in sys.modules:
+            return _untraced_form(fn)(*args, **kwargs)
+        return fn(*args, **kwargs)
+
+    return call
 
 
 def set_debug_flags(flags: int) -> int:
@@ -46,10 +73,14 @@ _first_use_status: dict = {}  # device index -> status word after the first-use 
 def _status_word(device: torch.device) -> torch.Tensor:
     key = device.index if device.index is not None else torch.cuda.current_device()
     w = _status_words.get(key)
-    if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
-        _status_words[key] = w
-        _first_use(torch.device("cuda", key), w)
+    return _new_status_word(key) if w is None else w
+
+
+@untraced
+def _new_status_word(key: int) -> torch.Tensor:
+    w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+    _status_words[key] = w
+    _first_use(torch.device("cuda", key), w)
     return w
 
 
@@ -66,7 +97,7 @@ def _first_use(device: torch.device, status: torch.Tensor) -> None:
     if torch.cuda.is_current_stream_capturing():
         return
     lib = _lib.load()
-    stream = _stream(device)
+    stream = torch.cuda.current_stream(device).cuda_stream
     with torch.cuda.device(device):
         for d in (64, 128):
             x = torch.ones(1, 160, 128, d, dtype=torch.bfloat16, device=device)  # a CTA on every SM
@@ -152,7 +183,7 @@ def _rows_call(name: str, src: torch.Tensor, dst: torch.Tensor, rows: int, d: in
     lib = _lib.load()
     with torch.cuda.device(src.device):
         rc = getattr(lib, name)(src.data_ptr(), dst.data_ptr(), rows, d, dpad,
-                                _stream(src.device))
+                                torch.cuda.current_stream(src.device).cuda_stream)
     if rc != 0:
         raise RuntimeError(f"flashlinear: {name} returned {rc}: {_lib.strerror(rc)}")
 
@@ -171,6 +202,7 @@ def _kernel_view(t: torch.Tensor) -> torch.Tensor:
     return view
 
 
+@untraced
 def kernel_view(t: torch.Tensor) -> torch.Tensor:
     """Public form of the repack: callers that run several passes over the same tensor (forward then
     backward) repack it once and hand the view to every pass."""
@@ -210,12 +242,6 @@ def _dtype_code(t: torch.Tensor) -> int:
     return _lib.FLA_DTYPE_F16 if t.dtype == torch.float16 else _lib.FLA_DTYPE_BF16
 
 
-def _stream(device: torch.device) -> int:
-    """Address of the current stream. (Inside torch.compile, which traces the Python route of a call piece by piece,
-    torch.cuda.current_stream() is an object that does not have it.)"""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
 def _desc(t: Optional[torch.Tensor]) -> FlaTensor:
     if t is None:
         return FlaTensor(None, 0, 0, 0)
@@ -236,7 +262,7 @@ def _call(pass_id: int, args: FlaArgs, device: torch.device, which: int = 0,
     caller hands in `workspace`; the scratch tensor (or None) is returned."""
     lib = _lib.load()
     with torch.cuda.device(device):
-        args.stream = _stream(device)
+        args.stream = torch.cuda.current_stream(device).cuda_stream
         args.status = _status_word(device).data_ptr()
         args.debug_flags = _debug_flags
         need = lib.fla_sm100_workspace_bytes(ctypes.byref(args), 0 if pass_id == 3 else pass_id)
@@ -370,6 +396,7 @@ def _product_sliced(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, like: tor
     return out
 
 
+@untraced
 def causal_dot_product_fwd(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -423,6 +450,7 @@ def causal_dot_product_fwd(
     return out
 
 
+@untraced
 def causal_dot_product_bwd(
     grad_output: torch.Tensor,
     q: torch.Tensor,
@@ -485,7 +513,7 @@ def causal_dot_product_bwd(
 def _norm_args(ref: torch.Tensor, dk: int, dv: int) -> FlaArgs:
     a = FlaArgs()
     a.batch, a.heads, a.seqlen, a.dk, a.dv = ref.shape[0], ref.shape[1], ref.shape[2], dk, dv
-    a.stream = _stream(ref.device)
+    a.stream = torch.cuda.current_stream(ref.device).cuda_stream
     a.status = _status_word(ref.device).data_ptr()
     return a
 
@@ -504,6 +532,7 @@ def _norm_check(rc: int, name: str) -> None:
         raise RuntimeError(f"flashlinear: {name} returned {rc}: {_lib.strerror(rc)}")
 
 
+@untraced
 def normalize_fwd(q: torch.Tensor, k: torch.Tensor, num: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
     """Divides `num` (the unnormalised product, [B,H,N,dv] bf16) IN PLACE by the denominator of
     README.md:27-30, den_i = q_i . sum_{j<=i} k_j + eps, and returns den as fp32 [B*H, N].
@@ -522,6 +551,7 @@ def normalize_fwd(q: torch.Tensor, k: torch.Tensor, num: torch.Tensor, eps: floa
     return den
 
 
+@untraced
 def normalize_bwd_prepare(g: torch.Tensor, out: torch.Tensor, den: torch.Tensor):
     """(dnum, dden) for upstream gradient g of the normalised output `out`: dnum = g / den (bf16,
     the upstream gradient of the unnormalised product), dden = -(g . out) / den (fp32 [B*H, N])."""
@@ -539,6 +569,7 @@ def normalize_bwd_prepare(g: torch.Tensor, out: torch.Tensor, den: torch.Tensor)
     return dnum, dden
 
 
+@untraced
 def normalize_bwd_sweep(q: torch.Tensor, k: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor,
                         dden: torch.Tensor) -> None:
     """Adds the denominator's gradient to dq and dk in place:
@@ -567,6 +598,7 @@ def normalized_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
         return _lib.load().fla_sm100_normalized_fused(ctypes.byref(a)) != 0
 
 
+@untraced
 def normalized_fwd(q, k, v, eps: float, need_grad: bool):
     """(out, den, s_final): the normalised output, its denominator (fp32 [B*H, N]) and, for a backward
     that has a use for it, the final state (else None)."""
@@ -588,6 +620,7 @@ def normalized_fwd(q, k, v, eps: float, need_grad: bool):
     return out, den, s_final
 
 
+@untraced
 def normalized_bwd(dnum, dden, q, k, v, s_last):
     """(dq, dk, dv) of the normalised attention from what normalize_bwd_prepare returned, with the denominator's
     part formed in the product kernel, or None for calls that take product and normalize_bwd_sweep instead."""
@@ -605,7 +638,7 @@ def normalized_bwd(dnum, dden, q, k, v, s_last):
     if not all(_addressable(t) for t in outs):
         return None
     with torch.cuda.device(q.device):
-        a.stream = _stream(q.device)
+        a.stream = torch.cuda.current_stream(q.device).cuda_stream
         a.status = _status_word(q.device).data_ptr()
         a.q, a.k, a.v, a.d_o = _desc(q), _desc(k), _desc(v), _desc(dnum)
         a.d_q, a.d_k, a.d_v = (_desc(t) for t in outs)
@@ -667,13 +700,14 @@ def _taylor_call(name: str, xq, xk, v, **tensors) -> None:
     for key, t in dict(tensors, q=_kernel_view(xq), k=_kernel_view(xk), v=_kernel_view(v)).items():
         setattr(args, key, _desc(t))
     with torch.cuda.device(xq.device):
-        args.stream = _stream(xq.device)
+        args.stream = torch.cuda.current_stream(xq.device).cuda_stream
         args.status = _status_word(xq.device).data_ptr()
         args.debug_flags = _debug_flags
         rc = getattr(_lib.load(), name)(ctypes.byref(args))
     _norm_check(rc, name)
 
 
+@untraced
 def taylor_forward(xq: torch.Tensor, xk: torch.Tensor, v: torch.Tensor) -> Optional[torch.Tensor]:
     """Causal linear attention on the Taylor features of raw q, k, formed on chip, or None for calls that
     have to go through taylor_features()."""
@@ -691,6 +725,7 @@ def taylor_forward(xq: torch.Tensor, xk: torch.Tensor, v: torch.Tensor) -> Optio
     return out
 
 
+@untraced
 def taylor_backward(grad_output: torch.Tensor, xq: torch.Tensor, xk: torch.Tensor, v: torch.Tensor):
     """Gradients of taylor_forward() with respect to xq, xk and v, or None as there."""
     g = grad_output
@@ -716,6 +751,7 @@ def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+@untraced
 def taylor_forward_in_memory(xq: torch.Tensor, xk: torch.Tensor, v: torch.Tensor):
     """(out, features of xq, features of xk): the same attention through features in memory."""
     native = _lib.host() if xq.is_cuda else None
@@ -730,6 +766,7 @@ def taylor_forward_in_memory(xq: torch.Tensor, xk: torch.Tensor, v: torch.Tensor
     return causal_dot_product_fwd(pq, pk, v), pq, pk
 
 
+@untraced
 def taylor_backward_in_memory(grad_output, xq, xk, v, pq, pk):
     """Gradients of taylor_forward_in_memory() with respect to xq, xk and v."""
     native = _lib.host() if xq.is_cuda else None
@@ -743,6 +780,7 @@ def taylor_backward_in_memory(grad_output, xq, xk, v, pq, pk):
     return taylor_features_bwd(dpq, xq), taylor_features_bwd(dpk, xk), dv
 
 
+@untraced
 def taylor_features(x: torch.Tensor) -> torch.Tensor:
     """Second-order Taylor features phi(x) = [1, x / d^(1/4), vec(x x^T) / (sqrt(2) sqrt(d))] of raw
     x [B, H, N, d] (bf16, d = 8 or 16): a [B, H, N, 1 + d + d^2] view of rows padded to a multiple
@@ -757,11 +795,12 @@ def taylor_features(x: torch.Tensor) -> torch.Tensor:
     buf = torch.empty(x.shape[:-1] + (fp.value,), dtype=x.dtype, device=x.device)
     with torch.cuda.device(x.device):
         rc = lib.fla_sm100_taylor_features(xc.data_ptr(), buf.data_ptr(), xc.numel() // d, d,
-                                           _stream(x.device))
+                                           torch.cuda.current_stream(x.device).cuda_stream)
     _norm_check(rc, "fla_sm100_taylor_features")
     return buf[..., :f.value]
 
 
+@untraced
 def taylor_features_bwd(dphi: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     """Gradient with respect to raw x of taylor_features(x) for feature gradients dphi
     ([B, H, N, 1 + d + d^2], rows padded to a multiple of 8 elements as taylor_features returns
@@ -783,7 +822,7 @@ def taylor_features_bwd(dphi: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     dx = torch.empty_like(xc)
     with torch.cuda.device(x.device):
         rc = lib.fla_sm100_taylor_features_bwd(dphi.data_ptr(), xc.data_ptr(), dx.data_ptr(), rows, d,
-                                               _stream(x.device))
+                                               torch.cuda.current_stream(x.device).cuda_stream)
     _norm_check(rc, "fla_sm100_taylor_features_bwd")
     return dx
 
@@ -822,6 +861,7 @@ def segment_states_buffer(q: torch.Tensor, v: torch.Tensor, segments: int = 0) -
     return torch.empty(need, dtype=torch.uint8, device=q.device)
 
 
+@untraced
 def chunk_state(b: torch.Tensor, c: torch.Tensor, segments: int = 0, keep_workspace: bool = False):
     """fp32 [batch*heads, db, dc] sum over tokens of b_j^T c_j: with (k, v) the forward state S of
     these tokens, with (q, dO) the backward state R. Used by sequence-sharded callers.

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import FlaRecurrenceArgs
-from .ops import _desc, _stream
+from .ops import _desc, untraced
 
 _DTYPES = {
     torch.bfloat16: _lib.FLA_DTYPE_BF16,
@@ -83,7 +83,7 @@ def _args(x: torch.Tensor, g: torch.Tensor) -> FlaRecurrenceArgs:
 
 def _call(name: str, a: FlaRecurrenceArgs, device: torch.device) -> None:
     with torch.cuda.device(device):
-        a.stream = _stream(device)
+        a.stream = torch.cuda.current_stream(device).cuda_stream
         a.status, a.debug_flags = ops._status_word(device).data_ptr(), ops._debug_flags
         rc = getattr(_lib.load(), name)(ctypes.byref(a))
     if rc != 0:
@@ -96,6 +96,7 @@ def _debug_check(device: torch.device) -> None:
         ops.check_status(device)
 
 
+@untraced
 def recurrence_fwd(
     x: torch.Tensor, log_decay: torch.Tensor, s_init: Optional[torch.Tensor] = None, keep_states: bool = False
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
@@ -128,6 +129,7 @@ def recurrence_fwd(
     return out, s_final, states
 
 
+@untraced
 def recurrence_bwd(
     grad_out: Optional[torch.Tensor],
     x: torch.Tensor,

@@ -50,9 +50,31 @@ def step(call, leaves):
     return [o.detach() for o in outs] + list(torch.autograd.grad(outs, leaves, ups))
 
 
+def attention():
+    fla = functions()
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    rand = lambda *s: torch.rand(*s, device=DEV, generator=gen).to(torch.bfloat16)  # noqa: E731
+    t = [rand(2, 3, 128, 64) for _ in range(3)]
+    odd = [rand(2, 3, 128, d) for d in (45, 45, 64)]
+    wide = [rand(2, 3, 128, d) for d in (273, 273, 16)]
+    raw = [rand(2, 3, 128, d) for d in (16, 16, 64)]
+    turned = [a.transpose(2, 3).contiguous().transpose(2, 3) for a in t]
+    return {
+        "attention": (lambda q, k, v: (fla.LinearAttention.apply(q * 2, k, v),), t),
+        "attention, columns apart": (lambda q, k, v: (fla.LinearAttention.apply(q * 2, k, v),), turned),
+        "attention, odd widths": (lambda q, k, v: (fla.LinearAttention.apply(q * 2, k, v),), odd),
+        "attention, wide": (lambda q, k, v: (fla.LinearAttentionSmallVHD.apply(q * 2, k, v),), wide),
+        "attention, a state": (lambda q, k, v: fla.LinearAttentionResumable.apply(q * 2, k, v, None), t),
+        "attention, normalised": (lambda q, k, v: (fla.LinearAttentionNormalized.apply(q * 2, k, v),), t),
+        "attention, normalised, odd widths": (lambda q, k, v: (fla.LinearAttentionNormalized.apply(q * 2, k, v),), odd),
+        "attention, Taylor": (lambda q, k, v: (fla.TaylorLinearAttention.apply(q * 2, k, v),), raw),
+    }
+
+
 @pytest.mark.parametrize("backend", ["eager", "aot_eager"])
 def test_single_functions(native, backend):
-    for name, (call, leaves) in single().items():
+    for name, (call, leaves) in {**single(), **attention()}.items():
+        torch._dynamo.reset()
         compiled = torch.compile(call, backend=backend)
         for _ in range(2):
             assert all(torch.equal(a, b) for a, b in zip(step(compiled, leaves), step(call, leaves))), name
@@ -82,3 +104,65 @@ def test_refusals(native):
             call(x)
         with pytest.raises(error, match="flashlinear"):
             torch.compile(call, backend="eager")(x)
+
+
+def test_what_a_call_makes_lives_until_the_library_has_it(native, monkeypatch):
+    """Such as a gate that is written out for all channels. Traced, a tensor is released when its address has been taken; allocations
+    before the launch, which this fills with NaN, then get its memory."""
+    from flashy_linear_attention_b200 import layer_norm, ops, recurrence
+
+    def spoiling(call):
+        def wrapper(*args, **kwargs):
+            spoil = [torch.full((2 * 3 * 128 * 64 // part,), torch.nan, device=DEV) for part in (1, 2, 4, 8) for _ in range(4)]
+            del spoil
+            return call(*args, **kwargs)
+
+        return wrapper
+
+    for module in (layer_norm, ops, recurrence):
+        monkeypatch.setattr(module, "_call", spoiling(module._call))
+    fla = functions()
+    w, b = torch.randn(64, device=DEV), torch.randn(64, device=DEV)
+    apart = lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2)  # noqa: E731
+    made = {
+        "recurrence": lambda t: fla.GatedLinearRecurrence.apply(t * 2, (-t.abs())[..., :1].expand_as(t))[0],
+        "recurrence, columns apart": lambda t: fla.GatedLinearRecurrence.apply(apart(t), -t.abs(), t[:, :, 0].half())[0],
+        "norm": lambda t: fla.LayerNorm.apply(apart(t), w.repeat(2)[::2], b),
+        "add_norm": lambda t: fla.AddLayerNorm.apply(t, apart(t), w, b.repeat(2)[::2])[0],
+        "attention": lambda t: fla.LinearAttention.apply(*(apart(a) for a in (t.bfloat16(), t.bfloat16().abs(), t.bfloat16()))),
+    }
+    for name, call in made.items():
+        torch._dynamo.reset()
+        compiled = torch.compile(call, backend="eager")
+        for n in (128, 64):
+            x = torch.randn(2, 3, n, 64, device=DEV)
+            grads = []
+            for f in (call, compiled):
+                leaf = x.clone().requires_grad_(True)
+                out = f(leaf)
+                out.float().sum().backward()
+                grads.append((out.detach(), leaf.grad))
+            assert all(torch.equal(a, b) for a, b in zip(*grads)), (name, n)
+
+
+@pytest.mark.parametrize("dynamic", [None, True])
+def test_calls_of_many_lengths(native, dynamic):
+    """More of them than are compiled for."""
+    fla = functions()
+    w, b = torch.randn(64, device=DEV), torch.randn(64, device=DEV)
+    made = {
+        "recurrence": lambda t: fla.GatedLinearRecurrence.apply(t * 2, (-t.abs())[..., :1].expand_as(t))[0],
+        "norm": lambda t: fla.LayerNorm.apply(t * 2, w, b),
+    }
+    for name, call in made.items():
+        torch._dynamo.reset()
+        compiled = torch.compile(call, backend="eager", dynamic=dynamic)
+        for n in range(1, 300, 23):
+            x = torch.randn(2, 3, n, 64, device=DEV)
+            grads = []
+            for f in (compiled, call):
+                leaf = x.clone().requires_grad_(True)
+                out = f(leaf)
+                out.sum().backward()
+                grads.append((out.detach(), leaf.grad))
+            assert all(torch.equal(a, b) for a, b in zip(*grads)), (name, n)
